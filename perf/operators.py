@@ -120,9 +120,10 @@ def _quantize_plain(x, block_rows):
     padded[:rows, :cols] = x
     blocks = padded.view(nr, block_rows, nc, BLOCK)
     amax = blocks.abs().amax(dim=(1, 3)).clamp(min=AMAX_FLOOR)
-    codes = (blocks * (E4M3_MAX / amax)[:, None, :, None]).view(nr * block_rows, nc * BLOCK)
+    top = torch.full_like(amax, E4M3_MAX)   # a tensor: torch replaces a division by a number by a product
+    codes = (blocks * (top / amax)[:, None, :, None]).view(nr * block_rows, nc * BLOCK)
     codes = codes[:rows, :_pad16(cols)].to(torch.float8_e4m3fn)
-    scales = amax / E4M3_MAX
+    scales = amax / top
     return codes, (scales.t().contiguous() if block_rows == 1 else scales)
 
 
