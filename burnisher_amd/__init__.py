@@ -135,6 +135,12 @@ SIGNATURES = {
     "bh_dit_workspace_bytes": ([_V], _I64),
     "bh_dit_position_table": ([_V, _V, _V], _I),
     "bh_dit_set_rows": ([_V, _I], _I),
+    "bh_quantize_fp8": ([_V, _I64, _V, _V, _I64, _I64, _I, _I, _V], _I),
+    "bh_gemm_fp8": ([_V, _V, _V, _V, _V, _V, _I64, _I64, _I64, _I, _I, _V, _I64, _V], _I),
+    "bh_gemm_fp8_workspace_bytes": ([_I64, _I64, _I64], _I64),
+    "bh_attention_window": ([_V, _I64, _V, _V, _I64, _V, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _I64,
+                             _I64, _I64, _V, _V, _I, _V, _I64, _V], _I),
+    "bh_attention_window_workspace_bytes": ([_I64] * 9, _I64),
     "bh_scale": ([_V, _V, _I64, _F, _I, _V], _I),
     "bh_timestep_embedding": ([_D, _I, _I64, _V, _I, _V], _I),
     "bh_probe_device": ([_V, _V, _I64, ctypes.POINTER(ProbeResult)], _I),

@@ -334,6 +334,156 @@ int bh_attention_strided(const void* q, int64_t ld_q, const void* k, const void*
                           head_dim, scale, nullptr, key_mask, mask_dtype, dtype, stream);
 }
 
+namespace {
+// A workspace that a caller passes: null, or aligned device memory of at least `need` bytes.
+float* checked_workspace(void* ws, int64_t bytes, int64_t need, const std::string& op) {
+    if (!ws || need == 0) return nullptr;
+    require(bytes >= need, op + ": the workspace holds " + std::to_string(bytes) + " bytes, this call needs " +
+                               std::to_string(need) + " (or none: NULL)");
+    require_device_ptr(ws, op.c_str(), "workspace");
+    require((reinterpret_cast<uintptr_t>(ws) & 15) == 0, op + ": the workspace is not 16-byte aligned");
+    return static_cast<float*>(ws);
+}
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+constexpr int64_t kSizeLimit = int64_t{1} << 30;   // of a matrix's rows and columns, and a sequence
+}  // namespace
+
+int bh_quantize_fp8(const void* x, int64_t ld_x, void* q, float* scales, int64_t rows, int64_t cols,
+                    int block_rows, int dtype, void* stream) {
+    return guarded([&] {
+        const char* op = "quantize_fp8 (hip-gfx950)";
+        require_nonneg(rows, op, "rows");
+        require_nonneg(cols, op, "cols");
+        require(block_rows == 1 || block_rows == 128, "quantize_fp8: block_rows must be 1 or 128");
+        require(ld_x >= cols, "quantize_fp8: ld_x is below cols");
+        require(rows < kSizeLimit && cols < kSizeLimit, "quantize_fp8: rows and cols must be below 2^30");
+        const bool f32 = is_f32(dtype);
+        if (rows == 0 || cols == 0) return;
+        require_device_ptr(x, op, "x");
+        require_device_ptr(q, op, "q");
+        require_device_ptr(scales, op, "scales");
+        require(aligned(q, 8), "quantize_fp8: q is not 8-byte aligned");
+        require(aligned(x, f32 ? 4 : 2) && aligned(scales, 4), "quantize_fp8: an operand is not aligned to its type");
+        ProfileScope ps(K_ELEMENTWISE, as_stream(stream), static_cast<double>(rows) * cols * (f32 ? 5 : 3));
+        launch_quantize_fp8(x, ld_x, static_cast<uint8_t*>(q), scales, rows, cols, block_rows == 128, f32,
+                            as_stream(stream));
+    });
+}
+
+int64_t bh_gemm_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+    int64_t bytes = -1;
+    (void)guarded([&] {
+        const char* op = "gemm_fp8 (hip-gfx950)";
+        require_nonneg(m, op, "m");
+        require_nonneg(n, op, "n");
+        require_nonneg(k, op, "k");
+        require(m < kSizeLimit && n < kSizeLimit && k < kSizeLimit, "gemm_fp8: m, n and k must be below 2^30");
+        bytes = m * n == 0 ? 0 : 4 * gemm_fp8_workspace_floats(m, n, k);
+    });
+    return bytes;
+}
+
+int bh_gemm_fp8(const void* a, const float* a_scales, const void* b, const float* b_scales,
+                const void* bias, void* out, int64_t m, int64_t n, int64_t k, int epilogue, int dtype,
+                void* workspace, int64_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        const char* op = "gemm_fp8 (hip-gfx950)";
+        require_nonneg(m, op, "m");
+        require_nonneg(n, op, "n");
+        require_nonneg(k, op, "k");
+        require(m < kSizeLimit && n < kSizeLimit && k < kSizeLimit, "gemm_fp8: m, n and k must be below 2^30");
+        require(epilogue >= BH_EPI_NONE && epilogue <= BH_EPI_SILU,
+                epilogue == BH_EPI_GELU_GATED ? "gemm_fp8 (hip-gfx950): GeluGated has no kernel here"
+                                              : "gemm_fp8 (hip-gfx950): unknown epilogue");
+        const bool f32 = is_f32(dtype);
+        if (m * n == 0) return;
+        require_device_ptr(a, op, "a");
+        require_device_ptr(a_scales, op, "a_scales");
+        require_device_ptr(b, op, "b");
+        require_device_ptr(b_scales, op, "b_scales");
+        optional_device_ptr(bias, op, "bias");
+        require_device_ptr(out, op, "out");
+        require(aligned(a, 16) && aligned(b, 16), "gemm_fp8: a and b must be 16-byte aligned");
+        require(aligned(a_scales, 4) && aligned(b_scales, 4) && aligned(bias, f32 ? 4 : 2) && aligned(out, f32 ? 4 : 2),
+                "gemm_fp8: an operand is not aligned to its type");
+        const int64_t need = 4 * gemm_fp8_workspace_floats(m, n, k);
+        float* ws = checked_workspace(workspace, workspace_bytes, need, "gemm_fp8");
+        launch_gemm_fp8(static_cast<const uint8_t*>(a), a_scales, static_cast<const uint8_t*>(b), b_scales, bias, out,
+                        m, n, k, epilogue, f32, ws, ws ? need / 4 : 0, as_stream(stream));
+    });
+}
+
+namespace {
+WindowShape window_shape(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                         int64_t head_dim, int64_t left, int64_t right, int64_t sinks) {
+    const char* op = "attention_window (hip-gfx950)";
+    require_nonneg(batch, op, "batch");
+    require_nonneg(heads, op, "heads");
+    require_nonneg(q_len, op, "q_len");
+    require_nonneg(kv_len, op, "kv_len");
+    require_nonneg(sinks, op, "sinks");
+    require(kv_heads > 0 && heads % kv_heads == 0, "attention_window: heads must be a multiple of kv_heads");
+    require(head_dim > 0 && head_dim <= 128 && head_dim % 8 == 0,
+            "attention_window (hip-gfx950): head_dim must be a multiple of 8 up to 128");
+    require(batch < kSizeLimit && heads < kSizeLimit && q_len < kSizeLimit && kv_len < kSizeLimit &&
+                heads / kv_heads * q_len < kSizeLimit,
+            "attention_window: kv_len and heads * q_len must be below 2^30");
+    auto side = [](int64_t w) { return w < 0 ? -1 : static_cast<int>(std::min(w, kSizeLimit)); };
+    return WindowShape{batch, heads, kv_heads, q_len, kv_len, head_dim, 0, 0, 0, 0.f, side(left), side(right),
+                       static_cast<int>(std::min(sinks, kSizeLimit))};
+}
+}  // namespace
+
+int64_t bh_attention_window_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
+                                            int64_t q_len, int64_t kv_len, int64_t head_dim,
+                                            int64_t window_left, int64_t window_right, int64_t sinks) {
+    int64_t bytes = -1;
+    (void)guarded([&] {
+        const WindowShape sh = window_shape(batch, heads, kv_heads, q_len, kv_len, head_dim, window_left, window_right,
+                                            sinks);
+        bytes = batch * heads * q_len == 0 ? 0 : 4 * attention_window_workspace_floats(sh);
+    });
+    return bytes;
+}
+
+int bh_attention_window(const void* q, int64_t ld_q, const void* k, const void* v, int64_t ld_kv,
+                        void* out, int64_t ld_out, int64_t batch, int64_t heads, int64_t kv_heads,
+                        int64_t q_len, int64_t kv_len, int64_t head_dim, float scale,
+                        int64_t window_left, int64_t window_right, int64_t sinks,
+                        const int32_t* kv_lens, const int32_t* q_starts, int dtype, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        const char* op = "attention_window (hip-gfx950)";
+        require(!is_f32(dtype), "attention_window (hip-gfx950): bf16 only");
+        WindowShape sh = window_shape(batch, heads, kv_heads, q_len, kv_len, head_dim, window_left, window_right, sinks);
+        require(ld_q >= heads * head_dim && ld_kv >= kv_heads * head_dim && ld_out >= heads * head_dim,
+                "attention_window: a row stride is below its heads * head_dim");
+        require(ld_q % 8 == 0 && ld_kv % 8 == 0 && ld_out % 4 == 0,
+                "attention_window: ld_q and ld_kv must be multiples of 8, ld_out of 4");
+        if (batch * heads * q_len == 0) return;
+        require_device_ptr(q, op, "q");
+        if (kv_len > 0) {
+            require_device_ptr(k, op, "k");
+            require_device_ptr(v, op, "v");
+        }
+        require_device_ptr(out, op, "out");
+        optional_device_ptr(kv_lens, op, "kv_lens");
+        optional_device_ptr(q_starts, op, "q_starts");
+        require(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 8),
+                "attention_window: q, k and v must be 16-byte, out 8-byte aligned");
+        require(aligned(kv_lens, 4) && aligned(q_starts, 4), "attention_window: an operand is not aligned to its type");
+        sh.ld_q = ld_q;
+        sh.ld_kv = ld_kv;
+        sh.ld_o = ld_out;
+        sh.scale = scale > 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(head_dim));
+        const int64_t need = 4 * attention_window_workspace_floats(sh);
+        float* ws = checked_workspace(workspace, workspace_bytes, need, "attention_window");
+        launch_attention_window(static_cast<const bf16_t*>(q), static_cast<const bf16_t*>(k),
+                                static_cast<const bf16_t*>(v), static_cast<bf16_t*>(out), sh, kv_lens, q_starts, ws,
+                                ws ? need / 4 : 0, as_stream(stream));
+    });
+}
+
 int bh_gather(const void* table, const float* ids, void* out, int64_t rows, int64_t cols,
               int64_t table_rows, int dtype, void* stream) {
     return guarded([&] {

@@ -550,4 +550,27 @@ void launch_adaln_chunks(const bf16_t* a, const bf16_t* w, const bf16_t* bias, c
 // ScaleArgs: out[i] = in[i] * scale, one rounding (out may alias in).
 void launch_scale(const void* in, void* out, int64_t n, float scale, bool f32, hipStream_t s);
 
+// ---- 8-bit matrices and windowed attention (quantize.hip, gemm_fp8.hip, window.hip) ----
+// Row stride in bytes of an e4m3 matrix of `cols` columns; the bytes from cols on are zero.
+__host__ __device__ inline int64_t fp8_row_bytes(int64_t cols) { return (cols + 15) & ~int64_t{15}; }
+// Codes and scales of x (rows of ld elements): a scale per row and 128 columns, [blocks of columns, rows],
+// or with `blocks` per 128 x 128, [blocks of rows, blocks of columns].
+void launch_quantize_fp8(const void* x, int64_t ld, uint8_t* q, float* scales, int64_t rows, int64_t cols, bool blocks,
+                         bool f32, hipStream_t s);
+// Floats of workspace with which a product of these sizes runs best (0: it uses none).
+int64_t gemm_fp8_workspace_floats(int64_t m, int64_t n, int64_t k);
+// bias and out are fp32 with f32, else bf16. `ws` of `ws_floats` (null: no workspace).
+void launch_gemm_fp8(const uint8_t* a, const float* sa, const uint8_t* b, const float* sb, const void* bias, void* out,
+                     int64_t m, int64_t n, int64_t k, int act, bool f32, float* ws, int64_t ws_floats, hipStream_t s);
+struct WindowShape {
+    int64_t batch, heads, kv_heads, q_len, kv_len, head_dim;
+    int64_t ld_q, ld_kv, ld_o;   // row strides in elements
+    float scale;                 // resolved (never <= 0)
+    int left, right, sinks;      // left, right: below 0 for no limit
+};
+int64_t attention_window_workspace_floats(const WindowShape& sh);
+void launch_attention_window(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16_t* out, const WindowShape& sh,
+                             const int32_t* kv_lens, const int32_t* q_starts, float* ws, int64_t ws_floats,
+                             hipStream_t s);
+
 }  // namespace bh

@@ -180,6 +180,68 @@ int bh_scale(const void* in, void* out, int64_t numel, float scale, int dtype, v
  * An odd dim is refused, as the reference refuses it. */
 int bh_timestep_embedding(double t, int dim, int64_t batch, void* out, int dtype, void* stream);
 
+/* ---- 8-bit matrices, and attention through a window ---------------------------------------- */
+
+/* Quantises x [rows, cols] (BH_F32 or BH_BF16, rows ld_x elements apart) to 8-bit floating point
+ * (e4m3: 4 exponent and 3 mantissa bits, largest value 448, no infinities) with one fp32 scale per
+ * block, so that x is about code * scale:
+ *   scale = max(amax, 2^-96) / 448, code = e4m3(x * (448 / max(amax, 2^-96))), amax = max |x|
+ * over the block, the product rounded to nearest even. It has no counterpart in the reference.
+ *   block_rows 1:   a block is 128 columns of one row (activations); scales is
+ *                   [ceil(cols / 128), rows];
+ *   block_rows 128: a block is 128 rows x 128 columns (weights); scales is
+ *                   [ceil(rows / 128), ceil(cols / 128)].
+ * The last blocks hold what is left. q's rows are round_up(cols, 16) bytes apart, and the bytes
+ * from cols on are written as zeros. A block that holds an infinity or a NaN gets a scale that is
+ * not finite, so every product with it is NaN. q is 8-byte aligned. */
+int bh_quantize_fp8(const void* x, int64_t ld_x, void* q, float* scales, int64_t rows, int64_t cols,
+                    int block_rows, int dtype, void* stream);
+
+/* The matrix product of two matrices as bh_quantize_fp8 writes them, a with block_rows 1 [m, k] and
+ * b with block_rows 128 [n, k] (a checkpoint's [out_features, in_features]):
+ *   out[m, n] = epilogue(sum_j a_scales[j, m] * b_scales[n / 128, j] * (a . b over block j) + bias[n])
+ * with bias and out in `dtype` and `epilogue` as in bh_gemm. Sums and scales are fp32. With a BH_F32
+ * output the codes are multiplied as bf16 values, exactly; with BH_BF16 by the 8-bit matrix
+ * instruction, which runs at twice the rate, adds eight neighbouring products at a time and drops of
+ * each what lies below 2^-13 of the largest of the eight (measured: about 2^-13 of the result, below
+ * the output's own 2^-8). a and b are 16-byte aligned and hold zeros from
+ * k to the end of each row.
+ * `workspace` is device memory of workspace_bytes, 16-byte aligned, that the call may write (partial
+ * sums of a split K): bh_gemm_fp8_workspace_bytes says how much a product uses, 0 for many. NULL
+ * runs without it (slower where it would be used; the sums then have another order); one that is too
+ * small is refused. A call reads nothing that an earlier one left there. Calls that overlap need
+ * workspaces of their own. Allocates nothing. */
+int bh_gemm_fp8(const void* a, const float* a_scales, const void* b, const float* b_scales,
+                const void* bias, void* out, int64_t m, int64_t n, int64_t k, int epilogue, int dtype,
+                void* workspace, int64_t workspace_bytes, void* stream);
+int64_t bh_gemm_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k);
+
+/* Attention through a sliding window, with first keys that stay visible and grouped heads; bf16.
+ * Query head h reads key head h / (heads / kv_heads). Query i of batch row b stands at position
+ * p = q_starts[b] + i and sees key j when
+ *   j < kv_lens[b] and j <= p + window_right and (j >= p - window_left or j < sinks);
+ * a window below 0 has no limit on its side, so window_right 0 is causal. kv_lens (NULL: kv_len) and
+ * q_starts (NULL: kv_len - q_len, the last queries of the sequence) are int32 [batch] on the device;
+ * a length is taken as at least 0 and at most kv_len. A query that sees no key gives zeros, unlike
+ * bh_attention, whose masked keys keep a score. Keys that no query of a batch row sees are not read
+ * into any sum, whatever they hold; a NaN or infinity in a key or value that one query sees may reach
+ * the queries near it. softmax(scale * q k^T) v with fp32 scores, scale <= 0 meaning 1/sqrt(head_dim).
+ * Element (b, s, h, d) of q lives at q[(b * q_len + s) * ld_q + h * head_dim + d], of k and v at
+ * [(b * kv_len + s) * ld_kv + h * head_dim + d] and of out with ld_out. head_dim is a multiple of 8
+ * up to 128, the row strides are multiples of 8 (ld_out of 4), q, k and v 16-byte and out 8-byte
+ * aligned, and kv_len and heads * q_len below 2^30.
+ * It has no counterpart in the reference. `workspace` as in bh_gemm_fp8: the partial results of keys
+ * split over workgroups (few queries, many keys). */
+int bh_attention_window(const void* q, int64_t ld_q, const void* k, const void* v, int64_t ld_kv,
+                        void* out, int64_t ld_out, int64_t batch, int64_t heads, int64_t kv_heads,
+                        int64_t q_len, int64_t kv_len, int64_t head_dim, float scale,
+                        int64_t window_left, int64_t window_right, int64_t sinks,
+                        const int32_t* kv_lens, const int32_t* q_starts, int dtype, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+int64_t bh_attention_window_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
+                                            int64_t q_len, int64_t kv_len, int64_t head_dim,
+                                            int64_t window_left, int64_t window_right, int64_t sinks);
+
 /* ---- device probe ---------------------------------------------------------------------------- */
 
 /* What the device sustains, measured by this library's own kernels (the reference's `probe`
