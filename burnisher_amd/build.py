@@ -64,6 +64,7 @@ def sources() -> list[Path]:
 EXTRA_FLAGS = {"flash72.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"],
                "cross_fused.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"],
                "flash512.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+               "gemm_fp8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                "denoise.hip": ["-ffp-contract=off"],
                "elementwise.hip": ["-ffp-contract=off"],
                "probe.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}

@@ -378,7 +378,8 @@ int64_t bh_gemm_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k) {
         require_nonneg(n, op, "n");
         require_nonneg(k, op, "k");
         require(m < kSizeLimit && n < kSizeLimit && k < kSizeLimit, "gemm_fp8: m, n and k must be below 2^30");
-        bytes = m * n == 0 ? 0 : 4 * gemm_fp8_workspace_floats(m, n, k);
+        if (m * n == 0) bytes = 0;
+        else bytes = 4 * std::max(gemm_fp8_workspace_floats(m, n, k, false), gemm_fp8_workspace_floats(m, n, k, true));
     });
     return bytes;
 }
@@ -406,10 +407,10 @@ int bh_gemm_fp8(const void* a, const float* a_scales, const void* b, const float
         require(aligned(a, 16) && aligned(b, 16), "gemm_fp8: a and b must be 16-byte aligned");
         require(aligned(a_scales, 4) && aligned(b_scales, 4) && aligned(bias, f32 ? 4 : 2) && aligned(out, f32 ? 4 : 2),
                 "gemm_fp8: an operand is not aligned to its type");
-        const int64_t need = 4 * gemm_fp8_workspace_floats(m, n, k);
+        const int64_t need = 4 * gemm_fp8_workspace_floats(m, n, k, f32);
         float* ws = checked_workspace(workspace, workspace_bytes, need, "gemm_fp8");
         launch_gemm_fp8(static_cast<const uint8_t*>(a), a_scales, static_cast<const uint8_t*>(b), b_scales, bias, out,
-                        m, n, k, epilogue, f32, ws, ws ? need / 4 : 0, as_stream(stream));
+                        m, n, k, epilogue, f32, ws, as_stream(stream));
     });
 }
 

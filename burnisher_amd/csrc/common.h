@@ -557,11 +557,11 @@ __host__ __device__ inline int64_t fp8_row_bytes(int64_t cols) { return (cols + 
 // or with `blocks` per 128 x 128, [blocks of rows, blocks of columns].
 void launch_quantize_fp8(const void* x, int64_t ld, uint8_t* q, float* scales, int64_t rows, int64_t cols, bool blocks,
                          bool f32, hipStream_t s);
-// Floats of workspace with which a product of these sizes runs best (0: it uses none).
-int64_t gemm_fp8_workspace_floats(int64_t m, int64_t n, int64_t k);
-// bias and out are fp32 with f32, else bf16. `ws` of `ws_floats` (null: no workspace).
+// Floats of workspace that a product of these sizes uses when it has one (0: none).
+int64_t gemm_fp8_workspace_floats(int64_t m, int64_t n, int64_t k, bool f32);
+// bias and out are fp32 with f32, else bf16. `ws`: those floats, or null to run without.
 void launch_gemm_fp8(const uint8_t* a, const float* sa, const uint8_t* b, const float* sb, const void* bias, void* out,
-                     int64_t m, int64_t n, int64_t k, int act, bool f32, float* ws, int64_t ws_floats, hipStream_t s);
+                     int64_t m, int64_t n, int64_t k, int act, bool f32, float* ws, hipStream_t s);
 struct WindowShape {
     int64_t batch, heads, kv_heads, q_len, kv_len, head_dim;
     int64_t ld_q, ld_kv, ld_o;   // row strides in elements

@@ -207,7 +207,8 @@ int bh_quantize_fp8(const void* x, int64_t ld_x, void* q, float* scales, int64_t
  * the output's own 2^-8). a and b are 16-byte aligned and hold zeros from
  * k to the end of each row.
  * `workspace` is device memory of workspace_bytes, 16-byte aligned, that the call may write (partial
- * sums of a split K): bh_gemm_fp8_workspace_bytes says how much a product uses, 0 for many. NULL
+ * sums of a split K): bh_gemm_fp8_workspace_bytes says how much a product of these sizes uses with
+ * either output type, 0 for many. NULL
  * runs without it (slower where it would be used; the sums then have another order); one that is too
  * small is refused. A call reads nothing that an earlier one left there. Calls that overlap need
  * workspaces of their own. Allocates nothing. */

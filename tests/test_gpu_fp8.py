@@ -213,6 +213,18 @@ def test_gemm_sizes(hip, m, n, k, dtype):
     check_gemm(m, n, k, dtype=dtype)
 
 
+# one and several blocks of K, one and several tiles a workgroup, K whole and in slices, on every tile
+TILE_SIZES = [(454, 3853, 16), (33, 39, 5011), (817, 4616, 170), (272, 3733, 3941), (929, 1287, 2911), (1843, 4127, 330),
+              (521, 3680, 4188), (2763, 2222, 200), (404, 4285, 5927), (1592, 802, 5735), (2256, 3619, 330),
+              (2951, 3411, 16), (2875, 4239, 330), (4500, 4300, 160), (2048, 2048, 2048)]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("m,n,k", TILE_SIZES)
+def test_gemm_tiles(hip, m, n, k, dtype):
+    check_gemm(m, n, k, dtype=dtype, with_bias=k % 2 == 1)
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("act", [0, 1, 2])
 @pytest.mark.parametrize("m,n,k", [(1, 300, 400), (40, 129, 256), (333, 640, 520), (2048, 256, 128)])
