@@ -461,6 +461,7 @@ int bh_attention_window(const void* q, int64_t ld_q, const void* k, const void* 
                 "attention_window: a row stride is below its heads * head_dim");
         require(ld_q % 8 == 0 && ld_kv % 8 == 0 && ld_out % 4 == 0,
                 "attention_window: ld_q and ld_kv must be multiples of 8, ld_out of 4");
+        require(ld_kv < (int64_t{1} << 24), "attention_window: ld_kv must be below 2^24");
         if (batch * heads * q_len == 0) return;
         require_device_ptr(q, op, "q");
         if (kv_len > 0) {
@@ -481,7 +482,7 @@ int bh_attention_window(const void* q, int64_t ld_q, const void* k, const void* 
         float* ws = checked_workspace(workspace, workspace_bytes, need, "attention_window");
         launch_attention_window(static_cast<const bf16_t*>(q), static_cast<const bf16_t*>(k),
                                 static_cast<const bf16_t*>(v), static_cast<bf16_t*>(out), sh, kv_lens, q_starts, ws,
-                                ws ? need / 4 : 0, as_stream(stream));
+                                as_stream(stream));
     });
 }
 

@@ -568,9 +568,9 @@ struct WindowShape {
     float scale;                 // resolved (never <= 0)
     int left, right, sinks;      // left, right: below 0 for no limit
 };
+// Floats of workspace that a call of this shape uses when it has one (0: none).
 int64_t attention_window_workspace_floats(const WindowShape& sh);
 void launch_attention_window(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16_t* out, const WindowShape& sh,
-                             const int32_t* kv_lens, const int32_t* q_starts, float* ws, int64_t ws_floats,
-                             hipStream_t s);
+                             const int32_t* kv_lens, const int32_t* q_starts, float* ws, hipStream_t s);
 
 }  // namespace bh

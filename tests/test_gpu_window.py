@@ -109,6 +109,25 @@ def test_self_attention_windows(hip, n, d, heads, kvh, left, right, sinks):
     check(2, heads, kvh, n, n, d, left, right, sinks, lens=[n, max(1, n // 3)], starts=[0, 0], seed=n)
 
 
+# enough rows to fill the chip: tiles of 128 rows
+@pytest.mark.parametrize("left,right,sinks", WINDOWS)
+@pytest.mark.parametrize("batch,n,d,heads,kvh", [(4, 150, 64, 32, 32), (4, 200, 128, 32, 8), (3, 333, 72, 15, 15)])
+def test_self_attention_windows_of_many_rows(hip, batch, n, d, heads, kvh, left, right, sinks):
+    lens = [n, n // 3, 1, 0][:batch]
+    check(batch, heads, kvh, n, n, d, left, right, sinks, lens=lens, starts=[0] * batch, seed=n)
+
+
+@pytest.mark.parametrize("d", [8, 16, 24, 32, 40, 48, 64, 72, 80, 88, 96, 104, 112, 120, 128])
+def test_head_dims_of_many_rows(hip, d):
+    check(8, 16, 16, 70, 90, d, 20, 5, 3, lens=[90, 89, 70, 64, 33, 90, 90, 12], starts=[20, 0, 0, 10, 3, -5, 40, 0])
+
+
+@pytest.mark.parametrize("n,heads,kvh", [(130, 32, 32), (70, 64, 16)])
+@pytest.mark.parametrize("poison", [math.nan, math.inf])
+def test_unseen_keys_never_enter_many_rows(hip, n, heads, kvh, poison):
+    check_poison(4, n, heads, kvh, poison)
+
+
 @pytest.mark.parametrize("d", [8, 16, 24, 32, 40, 48, 64, 72, 80, 88, 96, 104, 112, 120, 128])
 def test_head_dims(hip, d):
     check(1, 4, 2, 150, 150, d, 40, 0, 5)
@@ -166,12 +185,16 @@ def test_no_keys_at_all(hip):
 @pytest.mark.parametrize("n,heads", [(1, 8), (20, 2), (150, 2)])
 @pytest.mark.parametrize("poison", [math.nan, math.inf, -math.inf])
 def test_unseen_keys_never_enter(hip, n, heads, poison):
+    check_poison(2, n, heads, 2, poison)
+
+
+def check_poison(batch, n, heads, kvh, poison):
     import torch
     kv_len, left, sinks = 600, 90, 3
-    q, k, v = normal((2, n, heads, 64), 1), normal((2, kv_len, 2, 64), 2), normal((2, kv_len, 2, 64), 3)
-    lens = [500, 211]
+    q, k, v = normal((batch, n, heads, 64), 1), normal((batch, kv_len, kvh, 64), 2), normal((batch, kv_len, kvh, 64), 3)
+    lens = [500, 211, 600, 333][:batch]
     starts = [x - n for x in lens]
-    for b in range(2):
+    for b in range(batch):
         unseen = ~sees(torch.arange(n, device="cuda") + starts[b], lens[b], kv_len, left, 0, sinks).any(0)
         k[b, unseen], v[b, unseen] = poison, poison
     got = run(q, k, v, lens, starts, left, 0, sinks)

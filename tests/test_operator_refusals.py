@@ -74,7 +74,7 @@ def window(**over):
     (dict(k=D + 8), "16-byte"), (dict(v=D + 2), "16-byte"), (dict(out=D + 4), "8-byte"), (dict(lens=D + 2), "aligned to"),
     (dict(starts=D + 1), "aligned to"), (dict(sinks=-1), "sinks is negative"), (dict(q_len=-1), "q_len is negative"),
     (dict(kv_len=-1), "kv_len is negative"), (dict(batch=-1), "batch is negative"), (dict(kv_len=1 << 30), "2^30"),
-    (dict(q_len=1 << 29), "2^30")])
+    (dict(q_len=1 << 29), "2^30"), (dict(ld_kv=1 << 24), "2^24")])
 def test_window_refuses(over, says):
     assert says in window(**over)
 
