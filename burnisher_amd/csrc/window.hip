@@ -34,6 +34,7 @@ constexpr float kLowest = -3.4028235e38f;   // a maximum before any score: finit
 constexpr float kSlack = 8.0f;
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef short s16x8_t __attribute__((ext_vector_type(8)));
 
 struct WindowArgs {
@@ -129,7 +130,8 @@ struct Rows {
     static constexpr int KS = (DT + 1) / 2;   // K = 32 steps of the score product
     bf16x8_t q[QT][KS];
     f32x4_t o[DT][QT];                        // o[e][u][r]: column 16 e + 4 g + r
-    float top[QT], sum[QT];                   // the running maximum; this lane's part of the denominator
+    f32x4_t sum[QT];                          // the denominator, from a row of ones beside V^T: the matrix cores add it up
+    float top[QT];                            // the running maximum
     int lo[QT], hi[QT];                       // the row's window
 
     __device__ __forceinline__ void init(const WindowArgs& a, const Keys& keys, int b, int kh, int row0, int rows, int lane) {
@@ -148,48 +150,44 @@ struct Rows {
                 for (int e = 0; e < 8; ++e) q[u][ks][e] = d < a.D ? f[e] : static_cast<__bf16>(0.0f);
             }
             top[u] = kLowest;
-            sum[u] = 0.f;
+            sum[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < DT; ++e) o[e][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         }
     }
 
-    // Scores, weights and output sums of 16 T keys (T even) from `base` on in the LDS images at kp and vp. `masked`: some row
-    // sees only some of them.
-    template <int T>
-    __device__ __forceinline__ void step(const char* kp, const char* vp, int kpitch, int vpitch, int D, int base, int end,
-                                         int sinks, bool masked, float c_, int lane) {
+    // The scores of 16 keys, rows 16 t .. of the LDS image at kp: lane (g, c) has keys 16 t + 4 g + r of row c. Past
+    // head_dim the query is zero, against the key's last chunk again.
+    __device__ __forceinline__ void scores(f32x4_t (&s)[QT], int t, const char* kp, int kpitch, int D, int lane) const {
         const int g = lane >> 4, c = lane & 15;
-        f32x4_t s[T][QT];
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
+        for (int ks = 0; ks < KS; ++ks) {
+            const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kp + (t * 16 + c) * kpitch + min(ks * 64 + g * 16, D * 2 - 16));
 #pragma unroll
-            for (int u = 0; u < QT; ++u) s[t][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kp + (t * 16 + c) * kpitch + min(ks * 64 + g * 16, D * 2 - 16));
-                if (ks == KS - 1)   // past head_dim the query is zero, and so must the key be: it may hold a NaN
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) kf[e] = ks * 32 + g * 8 < D ? kf[e] : static_cast<__bf16>(0.0f);
-#pragma unroll
-                for (int u = 0; u < QT; ++u) s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[u][ks], s[t][u], 0, 0, 0);
-            }
+            for (int u = 0; u < QT; ++u)
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[u][ks], ks == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : s[u], 0, 0, 0);
         }
-        if (masked) {
+    }
+    // Those of keys from `base` on that a row does not see become -inf.
+    template <int T>
+    __device__ __forceinline__ void mask(f32x4_t (&s)[T][QT], int base, int end, int sinks, int lane) const {
+        const int g = lane >> 4;
 #pragma unroll
-            for (int u = 0; u < QT; ++u) {
-                const int first = lo[u] - base, last = min(hi[u], end) - base, near = sinks - base;
+        for (int u = 0; u < QT; ++u) {
+            const int first = lo[u] - base, last = min(hi[u], end) - base, near = sinks - base;
 #pragma unroll
-                for (int t = 0; t < T; ++t)
+            for (int t = 0; t < T; ++t)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int j = t * 16 + g * 4 + r;
-                        if (!(j < last && (j >= first || j < near))) s[t][u][r] = -INFINITY;
-                    }
-            }
+                for (int r = 0; r < 4; ++r) {
+                    const int j = t * 16 + g * 4 + r;
+                    const bool seen = (j < last) & ((j >= first) | (j < near));
+                    s[t][u][r] = seen ? s[t][u][r] : -INFINITY;
+                }
         }
-        float mx[QT];
-        bool move = false;
+    }
+    // The largest of this lane's scores of each row, in the maximum's units.
+    template <int T>
+    __device__ __forceinline__ void largest(float (&mx)[QT], const f32x4_t (&s)[T][QT], float c_) const {
 #pragma unroll
         for (int u = 0; u < QT; ++u) {
             mx[u] = -INFINITY;
@@ -198,141 +196,183 @@ struct Rows {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) mx[u] = fmaxf(mx[u], s[t][u][r]);
             mx[u] *= c_;
-            move |= mx[u] > top[u] + kSlack;
         }
-        if (__any(move)) {
+    }
+    // Moves the maximum, and with it the sums, where a score exceeds it by more than the slack.
+    __device__ __forceinline__ void raise(const float (&mx)[QT]) {
+        bool move = false;
 #pragma unroll
-            for (int u = 0; u < QT; ++u) {
-                float m = fmaxf(mx[u], __shfl_xor(mx[u], 16, 64));
-                m = fmaxf(m, __shfl_xor(m, 32, 64));
-                m = fmaxf(m, top[u]);
-                const float alpha = exp2f(top[u] - m);
-                top[u] = m;
-                sum[u] *= alpha;
+        for (int u = 0; u < QT; ++u) move |= mx[u] > top[u] + kSlack;
+        if (!__any(move)) return;
 #pragma unroll
-                for (int e = 0; e < DT; ++e)
+        for (int u = 0; u < QT; ++u) {
+            float m = fmaxf(mx[u], __shfl_xor(mx[u], 16, 64));
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            m = fmaxf(m, top[u]);
+            const float alpha = exp2f(top[u] - m);
+            top[u] = m;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) o[e][u][r] *= alpha;
-            }
+            for (int r = 0; r < 4; ++r) sum[u][r] *= alpha;
+#pragma unroll
+            for (int e = 0; e < DT; ++e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[e][u][r] *= alpha;
         }
+    }
+    // The weights of a score tile, in bf16: half an operand of the output product.
+    __device__ __forceinline__ u32x2_t weights(const f32x4_t& s, int u, float c_) const {
+        float w[4];
 #pragma unroll
-        for (int u = 0; u < QT; ++u)
+        for (int r = 0; r < 4; ++r) w[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c_, -top[u]));
+        return u32x2_t{f2bf2(w[0], w[1]), f2bf2(w[2], w[3])};
+    }
+    static __device__ __forceinline__ bf16x8_t operand(u32x2_t x, u32x2_t y) {
+        return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3));
+    }
+    // The output sums and denominators, V's image at vp.
+    template <int T>
+    __device__ __forceinline__ void accumulate(const bf16x8_t (&p)[T / 2][QT], const char* vp, int vpitch, int lane) {
+        const int g = lane >> 4, c = lane & 15;
+        bf16x8_t ones;
 #pragma unroll
-            for (int t = 0; t < T; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][u][r], c_, -top[u]));
-                    sum[u] += p;
-                    s[t][u][r] = p;
-                }
+        for (int e = 0; e < 8; ++e) ones[e] = static_cast<__bf16>(1.0f);
         const char* vrow = vp + (g * 4 + (c >> 2)) * vpitch + (c & 3) * 8;
 #pragma unroll
         for (int h = 0; h < T / 2; ++h) {
-            bf16x8_t p[QT];
-#pragma unroll
-            for (int u = 0; u < QT; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    p[u][r] = static_cast<__bf16>(s[2 * h][u][r]);
-                    p[u][4 + r] = static_cast<__bf16>(s[2 * h + 1][u][r]);
-                }
 #pragma unroll
             for (int e = 0; e < DT; ++e) {
                 const char* at = vrow + h * 32 * vpitch + e * 32;
                 const s16x8_t v = __builtin_shufflevector(read_transposed(at), read_transposed(at + 16 * vpitch), 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
                 for (int u = 0; u < QT; ++u)
-                    o[e][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v), p[u], o[e][u], 0, 0, 0);
+                    o[e][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v), p[h][u], o[e][u], 0, 0, 0);
             }
+#pragma unroll
+            for (int u = 0; u < QT; ++u) sum[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[h][u], sum[u], 0, 0, 0);
         }
-    }
-
-    __device__ __forceinline__ float denominator(int u) const {
-        float l = sum[u] + __shfl_xor(sum[u], 16, 64);
-        return l + __shfl_xor(l, 32, 64);
     }
 };
 
-// Whether a wave whose rows' windows run from [lo0, hi0) (its first token's) to [lo1, hi1) (its last's) sees something
-// of keys base .. base + N - 1, and whether all its rows see all of them.
-template <int N>
-__device__ __forceinline__ bool sees_some(int base, int end, int lo0, int hi1, int sinks) {
-    return base < min(end, hi1) && (base + N > lo0 || base < sinks);
-}
+// Whether rows whose windows run from [., hi0) (their first token's) to [lo1, .) (their last's) see all of keys
+// base .. base + N - 1.
 template <int N>
 __device__ __forceinline__ bool sees_all(int base, int end, int lo1, int hi0, int sinks) {
     return base + N <= min(end, hi0) && (base >= lo1 || base + N <= sinks);
 }
 
-// ---- many rows: 128 a workgroup, 32 a wave; K and V in blocks of 64 keys that its four waves share ------
+// ---- many rows: 128 a workgroup, 32 a wave; K and V in blocks of 64 keys that its four waves share --------
+//
+// Two workgroups a CU, each with two slots in LDS for K and for V; deeper rings, tiles of 256 rows and 32 x 32 x 16
+// products were no faster. What bounds it: the vector instructions, 32 exponentials (16 cycles each) and about 90 others
+// a lane and block, run beside the matrix ones only in part (2 x 16384 tokens of 16 heads, window 1024 to either side,
+// head_dim 64: vector 67%, matrix 38% of the time; head_dim 128: 46% and 46%).
 
-constexpr int kKeys = 64;
+constexpr int kKeys = 64, kManyRows = 128;
 
-template <int DT, int QT>
+template <int DT>
 __global__ void __launch_bounds__(kThreads, 2) k_window_many(WindowArgs a) {
-    constexpr int kChunks = DT * 2, KP = k_pitch(kChunks), VP = v_pitch(kChunks);   // for the widest head_dim here
-    constexpr int kStage = kKeys * 16 * (KP + VP);
-    constexpr int kItems = (KP + VP + 3) / 4;       // loads a wave issues per block
-    __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
+    constexpr int QT = 2, kChunks = DT * 2, KP = k_pitch(kChunks), VP = v_pitch(kChunks);   // for the widest head_dim here
+    constexpr int kKBytes = kKeys * 16 * KP, kVBytes = kKeys * 16 * VP;
+    constexpr int kKItems = (KP + 3) / 4, kVItems = (VP + 3) / 4;   // loads a wave issues per block, at most
+    __shared__ __attribute__((aligned(1024))) char kmem[2 * kKBytes], vmem[2 * kVBytes];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int T = a.tiles * a.B * a.KH;
     int id = blockIdx.x;
     if ((T & 7) == 0) id = (id & 7) * (T >> 3) + (id >> 3);   // neighbouring tiles, which share keys, on one XCD
     const int tile = id % a.tiles, bk = id / a.tiles, kh = bk % a.KH, b = bk / a.KH;
-    const int rows = a.group * a.Sq, row0 = tile * (64 * QT), row1 = min(row0 + 64 * QT, rows) - 1;
+    const int rows = a.group * a.Sq, row0 = tile * kManyRows, row1 = min(row0 + kManyRows, rows) - 1;
     const Keys keys(a, b, row0 / a.group, row1 / a.group);
     const Blocks<kKeys> blocks(keys);
 
     Rows<DT, QT> w;
     const int w0 = row0 + wave * (16 * QT), w1 = min(w0 + 16 * QT, rows) - 1;
     w.init(a, keys, b, kh, w0, rows, lane);
-    const bool any = w0 < rows;
     const int t0 = min(w0, rows - 1) / a.group, t1 = max(w1, 0) / a.group;
-    const int lo0 = keys.see_lo(a, t0), lo1 = keys.see_lo(a, t1), hi0 = keys.see_hi(a, t0), hi1 = keys.see_hi(a, t1);
+    const int lo0 = keys.see_lo(a, t0), lo1 = keys.see_lo(a, t1), hi0 = keys.see_hi(a, t0);
+    const int hi1 = w0 < rows ? keys.see_hi(a, t1) : 0;   // a wave without rows sees nothing
 
     const uint32_t ld_bytes = static_cast<uint32_t>(a.ld_kv) * 2;
     const int chunks = a.D / 8;
     const int64_t first = static_cast<int64_t>(b) * a.Skv * a.ld_kv + static_cast<int64_t>(kh) * a.D;
-    // item i of a wave: LDS rows of 1 KiB 4 i + wave, K's first, then V's
-    uint32_t off[kItems];
+    // a wave's loads of a block: rows 4 i + wave of 1 KiB of its LDS image
+    uint32_t koff[kKItems], voff[kVItems];
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-        const int n = i * 4 + wave;
-        off[i] = n < KP ? chunk_offset<KP>(n, lane, chunks, kKeys - 1, ld_bytes)
-                        : chunk_offset<VP>(n - KP, lane, chunks, kKeys - 1, ld_bytes);
-    }
-    auto load = [&](int j) {
-        char* stage = smem + (j & 1) * kStage;
+    for (int i = 0; i < kKItems; ++i) koff[i] = chunk_offset<KP>(i * 4 + wave, lane, chunks, kKeys - 1, ld_bytes);
+#pragma unroll
+    for (int i = 0; i < kVItems; ++i) voff[i] = chunk_offset<VP>(i * 4 + wave, lane, chunks, kKeys - 1, ld_bytes);
+    auto load_k = [&](int j) {
         const int base = blocks.base(j), last = blocks.end(j) - base - 1;
-        const bf16_t *k = a.k + first + static_cast<int64_t>(base) * a.ld_kv, *v = a.v + first + static_cast<int64_t>(base) * a.ld_kv;
+        const bf16_t* k = a.k + first + static_cast<int64_t>(base) * a.ld_kv;
 #pragma unroll
-        for (int i = 0; i < kItems; ++i) {
+        for (int i = 0; i < kKItems; ++i) {
             const int n = i * 4 + wave;
-            if (n >= KP + VP) continue;
-            uint32_t o = off[i];
-            if (last < kKeys - 1)
-                o = n < KP ? chunk_offset<KP>(n, lane, chunks, last, ld_bytes) : chunk_offset<VP>(n - KP, lane, chunks, last, ld_bytes);
-            dma16(n < KP ? k : v, o, stage + n * 1024);
+            if (n < KP) dma16(k, last < kKeys - 1 ? chunk_offset<KP>(n, lane, chunks, last, ld_bytes) : koff[i], kmem + (j & 1) * kKBytes + n * 1024);
         }
     };
-    if (blocks.n > 0) load(0);
-    for (int j = 0; j < blocks.n; ++j) {
-        // block j has landed, for everyone behind the barrier, and everyone has read block j - 1
+    auto load_v = [&](int j) {
+        const int base = blocks.base(j), last = blocks.end(j) - base - 1;
+        const bf16_t* v = a.v + first + static_cast<int64_t>(base) * a.ld_kv;
+#pragma unroll
+        for (int i = 0; i < kVItems; ++i) {
+            const int n = i * 4 + wave;
+            if (n < VP) dma16(v, last < kKeys - 1 ? chunk_offset<VP>(n, lane, chunks, last, ld_bytes) : voff[i], vmem + (j & 1) * kVBytes + n * 1024);
+        }
+    };
+    auto join = [&]() {   // this wave's loads have landed and its reads are done; behind the barrier everyone's
         asm volatile("" ::: "memory");
         s_waitcnt<0, 0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (j + 1 < blocks.n) load(j + 1);
+    };
+    f32x4_t s[4][QT];
+    float mx[QT];
+    auto seen = [&](int j) {   // some row of the wave sees some key of the block
+        const int base = blocks.base(j);
+        return j < blocks.n && base < min(blocks.end(j), hi1) && (base + kKeys > lo0 || base < a.sinks);
+    };
+    auto maximum = [&](int j) {
         const int base = blocks.base(j), end = blocks.end(j);
-        if (!any || !sees_some<kKeys>(base, end, lo0, hi1, a.sinks)) continue;
-        const char* stage = smem + (j & 1) * kStage;
-        w.template step<4>(stage, stage + KP * 1024, KP * 16, VP * 16, a.D, base, end, a.sinks,
-                           !sees_all<kKeys>(base, end, lo1, hi0, a.sinks), a.c, lane);
+        if (!sees_all<kKeys>(base, end, lo1, hi0, a.sinks)) w.template mask<4>(s, base, end, a.sinks, lane);
+        w.template largest<4>(mx, s, a.c);
+        w.raise(mx);
+    };
+    if (blocks.n > 0) {
+        load_k(0);
+        load_v(0);
+        join();
+        if (blocks.n > 1) load_k(1);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) w.scores(s[t], t, kmem, KP * 16, a.D, lane);
+        maximum(0);
+    }
+    // Block j's weights beside block j + 1's score product, which takes their place tile by tile, then block j's output
+    // product. Behind the barrier K of block j + 1 and V of block j have landed, and K of block j and V of block j - 1
+    // have been read. Scores that no row of the wave sees are -inf here, so a block that it does not see adds nothing.
+    for (int j = 0; j < blocks.n; ++j) {
+        join();
+        if (j + 2 < blocks.n) load_k(j + 2);
+        if (j + 1 < blocks.n) load_v(j + 1);
+        if (!seen(j) && !seen(j + 1)) continue;
+        const char* kp = kmem + ((j + 1) & 1) * kKBytes;   // behind the last block: scores that nobody uses
+        u32x2_t half[4][QT];
+        bf16x8_t p[2][QT];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int u = 0; u < QT; ++u) half[t][u] = w.weights(s[t][u], u, a.c);
+            w.scores(s[t], t, kp, KP * 16, a.D, lane);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int u = 0; u < QT; ++u) p[h][u] = w.operand(half[2 * h][u], half[2 * h + 1][u]);
+        w.template accumulate<4>(p, vmem + (j & 1) * kVBytes, VP * 16, lane);
+        if (j + 1 < blocks.n) maximum(j + 1);
     }
     const int g = lane >> 4, c = lane & 15;
 #pragma unroll
     for (int u = 0; u < QT; ++u) {
-        const float l = w.denominator(u);
+        const float l = w.sum[u][0];
         const int row = w0 + u * 16 + c;
         if (row >= rows) continue;
         const float rl = l == 0.f ? 0.f : 1.0f / l;
@@ -348,14 +388,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_window_many(WindowArgs a) {
     }
 }
 
-// ---- few rows: 16 a workgroup, whose waves take pieces of 32 keys in turn, each through LDS of its own -----
+// ---- few rows: 16 QT a workgroup, whose waves take pieces of 32 keys in turn, each through LDS of its own ----
 //
 // Bound by the keys' bytes: a wave waits only for its own loads, two pieces in flight, and the waves' sums meet
 // at the end. With `splits` the keys go to several workgroups, whose partial results k_window_join sums.
 
 constexpr int kPiece = 32;
 
-template <int DT>
+template <int DT, int QT>
 __global__ void __launch_bounds__(kThreads, 1) k_window_few(WindowArgs a) {
     constexpr int kChunks = DT * 2, KP = k_pitch(kChunks), VP = v_pitch(kChunks);
     constexpr int kK = (KP + 1) / 2, kItems = kK + VP / 2;   // loads per piece: 32 rows of KP and of VP chunks
@@ -363,9 +403,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_window_few(WindowArgs a) {
     static_assert(kItems <= 60, "vmcnt");
     __shared__ __attribute__((aligned(1024))) char smem[4 * 2 * kStage];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int split = blockIdx.x % a.splits, id = blockIdx.x / a.splits;
-    const int tile = id % a.tiles, bk = id / a.tiles, kh = bk % a.KH, b = bk / a.KH;
-    const int rows = a.group * a.Sq, row0 = tile * 16, row1 = min(row0 + 16, rows) - 1;
+    const int T = gridDim.x;
+    int id = blockIdx.x;
+    if ((T & 7) == 0) id = (id & 7) * (T >> 3) + (id >> 3);   // tiles that read the same keys on one XCD
+    const int tile = id % a.tiles, split = id / a.tiles % a.splits, bk = id / a.tiles / a.splits, kh = bk % a.KH, b = bk / a.KH;
+    const int rows = a.group * a.Sq, row0 = tile * (16 * QT), row1 = min(row0 + 16 * QT, rows) - 1;
     const int t0 = row0 / a.group, t1 = row1 / a.group;
     const Keys keys(a, b, t0, t1);
     const Blocks<kPiece> pieces(keys);
@@ -373,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_window_few(WindowArgs a) {
     const int j1 = static_cast<int>(static_cast<int64_t>(split + 1) * pieces.n / a.splits);
     const int lo1 = keys.see_lo(a, t1), hi0 = keys.see_hi(a, t0);
 
-    Rows<DT, 1> w;
+    Rows<DT, QT> w;
     const uint32_t ld_bytes = static_cast<uint32_t>(a.ld_kv) * 2;
     const int chunks = a.D / 8;
     const int64_t first = static_cast<int64_t>(b) * a.Skv * a.ld_kv + static_cast<int64_t>(kh) * a.D;
@@ -406,8 +448,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_window_few(WindowArgs a) {
         asm volatile("" ::: "memory");
         const int base = pieces.base(j), end = pieces.end(j);
         const char* stage = own + slot * kStage;
-        w.template step<2>(stage, stage + kK * 1024, KP * 16, VP * 16, a.D, base, end, a.sinks,
-                           !sees_all<kPiece>(base, end, lo1, hi0, a.sinks), a.c, lane);
+        f32x4_t s[2][QT];
+        float mx[QT];
+        bf16x8_t p[1][QT];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) w.scores(s[t], t, stage, KP * 16, a.D, lane);
+        if (!sees_all<kPiece>(base, end, lo1, hi0, a.sinks)) w.template mask<2>(s, base, end, a.sinks, lane);
+        w.template largest<2>(mx, s, a.c);
+        w.raise(mx);
+#pragma unroll
+        for (int u = 0; u < QT; ++u) p[0][u] = w.operand(w.weights(s[0][u], u, a.c), w.weights(s[1][u], u, a.c));
+        w.template accumulate<2>(p, stage + kK * 1024, VP * 16, lane);
         if (j + 8 < j1) {   // into the piece that was just read
             asm volatile("" ::: "memory");
             s_waitcnt<63, 0>();
@@ -417,45 +468,51 @@ __global__ void __launch_bounds__(kThreads, 1) k_window_few(WindowArgs a) {
         slot ^= 1;
     }
     // the four waves' rows: maximum, denominator and sums
-    constexpr int kRow = DT * 16 + 4;   // floats
-    static_assert(4 * 16 * kRow * 4 <= 4 * 2 * kStage, "the sums fit where the keys were");
-    const float l = w.denominator(0);
+    constexpr int kRows = 16 * QT, kRow = DT * 16 + 4;   // floats
+    static_assert(4 * kRows * kRow * 4 <= 4 * 2 * kStage, "the sums fit where the keys were");
     __syncthreads();
     float* sums = reinterpret_cast<float*>(smem);
     const int g = lane >> 4, c = lane & 15;
-    float* mine = sums + (wave * 16 + c) * kRow;
-    if (g == 0) {
-        mine[DT * 16] = w.top[0];
-        mine[DT * 16 + 1] = l;
-    }
 #pragma unroll
-    for (int e = 0; e < DT; ++e) *reinterpret_cast<f32x4_t*>(mine + e * 16 + g * 4) = w.o[e][0];
+    for (int u = 0; u < QT; ++u) {
+        float* mine = sums + (wave * kRows + u * 16 + c) * kRow;
+        if (g == 0) {
+            mine[DT * 16] = w.top[u];
+            mine[DT * 16 + 1] = w.sum[u][0];
+        }
+#pragma unroll
+        for (int e = 0; e < DT; ++e) *reinterpret_cast<f32x4_t*>(mine + e * 16 + g * 4) = w.o[e][u];
+    }
     __syncthreads();
-    const int r = threadIdx.x >> 4, row = row0 + r;
-    if (row >= rows) return;
-    float m = kLowest, total = 0.f, scale[4];
+    const int64_t all = static_cast<int64_t>(a.B) * a.KH * rows;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) m = fmaxf(m, sums[(k * 16 + r) * kRow + DT * 16]);
+    for (int u = 0; u < QT; ++u) {
+        const int r = u * 16 + (threadIdx.x >> 4), row = row0 + r;
+        if (row >= rows) return;
+        float m = kLowest, total = 0.f, scale[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        scale[k] = exp2f(sums[(k * 16 + r) * kRow + DT * 16] - m);
-        total += scale[k] * sums[(k * 16 + r) * kRow + DT * 16 + 1];
-    }
-    const int64_t all = static_cast<int64_t>(a.B) * a.KH * rows, at = static_cast<int64_t>(bk) * rows + row;
-    const float rl = total == 0.f ? 0.f : 1.0f / total;
-    bf16_t* dst = a.out + (static_cast<int64_t>(b) * a.Sq + row / a.group) * a.ld_o +
-                  static_cast<int64_t>(kh * a.group + row % a.group) * a.D;
-    for (int d = (threadIdx.x & 15) * 4; d < a.D; d += 64) {
-        f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < 4; ++k) m = fmaxf(m, sums[(k * kRows + r) * kRow + DT * 16]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v += *reinterpret_cast<const f32x4_t*>(sums + (k * 16 + r) * kRow + d) * scale[k];
-        if (a.splits == 1) *reinterpret_cast<uint2*>(dst + d) = make_uint2(f2bf2(v[0] * rl, v[1] * rl), f2bf2(v[2] * rl, v[3] * rl));
-        else *reinterpret_cast<f32x4_t*>(a.part + (split * all + at) * a.D + d) = v;
-    }
-    if (a.splits > 1 && (threadIdx.x & 15) == 0) {
-        float* ml = a.part + a.splits * all * a.D + (split * all + at) * 2;
-        ml[0] = m;
-        ml[1] = total;
+        for (int k = 0; k < 4; ++k) {
+            scale[k] = exp2f(sums[(k * kRows + r) * kRow + DT * 16] - m);
+            total += scale[k] * sums[(k * kRows + r) * kRow + DT * 16 + 1];
+        }
+        const int64_t at = static_cast<int64_t>(bk) * rows + row;
+        const float rl = total == 0.f ? 0.f : 1.0f / total;
+        bf16_t* dst = a.out + (static_cast<int64_t>(b) * a.Sq + row / a.group) * a.ld_o +
+                      static_cast<int64_t>(kh * a.group + row % a.group) * a.D;
+        for (int d = (threadIdx.x & 15) * 4; d < a.D; d += 64) {
+            f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v += *reinterpret_cast<const f32x4_t*>(sums + (k * kRows + r) * kRow + d) * scale[k];
+            if (a.splits == 1) *reinterpret_cast<uint2*>(dst + d) = make_uint2(f2bf2(v[0] * rl, v[1] * rl), f2bf2(v[2] * rl, v[3] * rl));
+            else *reinterpret_cast<f32x4_t*>(a.part + (split * all + at) * a.D + d) = v;
+        }
+        if (a.splits > 1 && (threadIdx.x & 15) == 0) {
+            float* ml = a.part + a.splits * all * a.D + (split * all + at) * 2;
+            ml[0] = m;
+            ml[1] = total;
+        }
     }
 }
 
@@ -496,28 +553,63 @@ int device_cus() {
     return n;
 }
 
+// How a call runs: k_window_many, or k_window_few on tiles of 16 `few` rows with the keys in `splits`. The estimates, in
+// us, were fitted to 20 shapes on one MI355X (head_dim 64 to 128, 1 to 2000 rows of 300 to 16000 keys), each on every
+// kernel and split that fits it; what they choose is within 6% of the fastest there but for 1.14 once (4 x 2 key heads x
+// 1200 rows, window 64: 13.0 against 11.4). Beside 3.5 a workgroup,
+//  - many: a block of 64 keys costs 0.62 + 0.006 head_dim alone on a CU, 0.5 + 0.014 beside another workgroup;
+//  - few: a piece of 32 keys for each of the four waves costs 0.35 + 0.005 head_dim on 16 rows, 0.3 + 0.009 on 32,
+//    0.35 + 0.0165 on 64, one workgroup a CU (two up to head_dim 64), and no less in all than reading the keys at
+//    5.2 TB/s (a quarter more on fewer workgroups than CUs);
+//  - a join costs 3 + 0.25 a split and its partial results at 3 TB/s.
+// 16 sequences of a token each, 32 / 8 heads of 128, 4096 keys: two splits 57 us, none 65, k_window_many 90. Four times
+// 64 tokens of the same: 32-row tiles 54, 16-row 82, 64-row 80, k_window_many 97. 2 x 64 heads of 300 tokens, head_dim 64:
+// k_window_many 15.6, 32-row tiles 24.
 struct Plan {
-    bool many;
+    int few;      // 0: k_window_many
     int splits;
 };
 Plan plan(const WindowShape& sh, bool may_split) {
-    const int64_t cus = device_cus(), group = sh.heads / sh.kv_heads, rows = group * sh.q_len;
-    const int64_t many = sh.batch * sh.kv_heads * ((rows + 127) / 128);
-    if (many * 2 >= cus) return {true, 1};
-    // the keys that 16 rows see at most, in pieces
-    const int64_t tokens = (15 + group) / group;
-    int64_t keys = sh.kv_len;
-    if (sh.left >= 0 && sh.right >= 0) keys = std::min(keys, static_cast<int64_t>(sh.left) + sh.right + tokens + sh.sinks);
-    const int64_t few = sh.batch * sh.kv_heads * ((rows + 15) / 16), pieces = (keys + kPiece - 1) / kPiece;
-    const int64_t splits = may_split ? std::min(std::max<int64_t>(1, 2 * cus / few), std::max<int64_t>(1, pieces / 8)) : 1;
-    return {false, static_cast<int>(std::min<int64_t>(splits, 64))};
+    const int64_t cus = device_cus(), group = sh.heads / sh.kv_heads, rows = group * sh.q_len, heads = sh.batch * sh.kv_heads;
+    const double D = static_cast<double>(sh.head_dim);
+    auto keys = [&](int64_t n) {   // that n rows see at most
+        if (sh.left < 0 || sh.right < 0) return sh.kv_len;
+        const int64_t tokens = std::min((n + group - 2) / group + 1, sh.q_len);
+        return std::min<int64_t>(sh.kv_len, int64_t{sh.left} + sh.right + tokens + sh.sinks);
+    };
+    auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    Plan best{0, 1};
+    double least = 1e30;
+    if (rows > 16) {
+        const int64_t groups = heads * up(rows, kManyRows);
+        const double blocks = static_cast<double>(up(keys(kManyRows), kKeys));
+        least = groups <= cus ? 3.5 + blocks * (0.62 + 0.006 * D) : up(groups, 2 * cus) * (3.5 + blocks * (0.5 + 0.014 * D));
+    }
+    for (int few : {1, 2, 4}) {
+        if (few > 1 && rows <= 8 * few) continue;
+        const int64_t pieces = up(keys(16 * few), kPiece);
+        const double step = few == 1 ? 0.35 + 0.005 * D : few == 2 ? 0.3 + 0.009 * D : 0.35 + 0.0165 * D;
+        for (int s = 1; s == 1 || (may_split && s <= 32 && 4 * s <= pieces); s *= 2) {
+            const int64_t groups = heads * up(rows, 16 * few) * s, at_once = cus * (sh.head_dim <= 64 ? 2 : 1);
+            const double bytes = static_cast<double>(heads) * keys(rows) * D * 4;
+            double cost = std::max(up(groups, at_once) * (3.5 + up(pieces, 4 * s) * step), bytes / 5.2e6 * (groups < cus ? 1.25 : 1.0));
+            if (s > 1) cost += 3 + 0.25 * s + s * static_cast<double>(heads) * rows * (D + 2) * 8 / 3e6;
+            if (cost < least) {
+                least = cost;
+                best = Plan{few, s};
+            }
+        }
+    }
+    return best;
 }
 
 template <int DT>
-void launch(const WindowArgs& a0, const Plan& how, int64_t grid, hipStream_t s) {
-    WindowArgs a = a0;
-    if (how.many) k_window_many<DT, 2><<<static_cast<unsigned>(grid), kThreads, 0, s>>>(a);
-    else k_window_few<DT><<<static_cast<unsigned>(grid), kThreads, 0, s>>>(a);
+void launch(const WindowArgs& a, const Plan& how, int64_t grid, hipStream_t s) {
+    const unsigned n = static_cast<unsigned>(grid);
+    if (how.few == 0) k_window_many<DT><<<n, kThreads, 0, s>>>(a);
+    else if (how.few == 1) k_window_few<DT, 1><<<n, kThreads, 0, s>>>(a);
+    else if (how.few == 2) k_window_few<DT, 2><<<n, kThreads, 0, s>>>(a);
+    else k_window_few<DT, 4><<<n, kThreads, 0, s>>>(a);
 }
 
 }  // namespace
@@ -541,7 +633,7 @@ void launch_attention_window(const bf16_t* q, const bf16_t* k, const bf16_t* v, 
     a.left = sh.left; a.right = sh.right; a.sinks = sh.sinks;
     a.c = sh.scale * kLog2e;
     const Plan how = plan(sh, ws != nullptr);
-    const int64_t rows = static_cast<int64_t>(a.group) * a.Sq, per = how.many ? 128 : 16, tiles = (rows + per - 1) / per;
+    const int64_t rows = static_cast<int64_t>(a.group) * a.Sq, per = how.few == 0 ? kManyRows : 16 * how.few, tiles = (rows + per - 1) / per;
     a.tiles = static_cast<int>(tiles);
     a.splits = how.splits;
     const int64_t grid = tiles * sh.batch * sh.kv_heads * how.splits;

@@ -122,6 +122,17 @@ def test_head_dims_of_many_rows(hip, d):
     check(8, 16, 16, 70, 90, d, 20, 5, 3, lens=[90, 89, 70, 64, 33, 90, 90, 12], starts=[20, 0, 0, 10, 3, -5, 40, 0])
 
 
+# tiles of 16, 32, 64 and 128 rows, the keys whole and split, at every width
+@pytest.mark.parametrize("d", [24, 64, 72, 88, 128])
+@pytest.mark.parametrize("heads,kvh,n,kv_len,left,right,sinks", [
+    (4, 4, 4, 1500, -1, 0, 0), (40, 8, 33, 300, 300, 300, 0), (40, 8, 70, 300, -1, 0, 0), (8, 8, 33, 1500, -1, 0, 0),
+    (8, 8, 33, 5000, -1, -1, 0), (40, 8, 33, 3000, -1, 0, 0), (40, 8, 70, 300, 20, 0, 4), (40, 8, 150, 300, 200, 20, 0),
+    (12, 4, 150, 300, 10, 0, 70)])
+def test_row_tiles_and_splits(hip, d, heads, kvh, n, kv_len, left, right, sinks):
+    lens = [kv_len, kv_len // 2, n]
+    check(3, heads, kvh, n, kv_len, d, left, right, sinks, lens=lens, starts=[x - n for x in lens], seed=d)
+
+
 @pytest.mark.parametrize("n,heads,kvh", [(130, 32, 32), (70, 64, 16)])
 @pytest.mark.parametrize("poison", [math.nan, math.inf])
 def test_unseen_keys_never_enter_many_rows(hip, n, heads, kvh, poison):
