@@ -398,10 +398,12 @@ int bh_gemm_fp8(const void* a, const float* a_scales, const void* b, const float
                                               : "gemm_fp8 (hip-gfx950): unknown epilogue");
         const bool f32 = is_f32(dtype);
         if (m * n == 0) return;
-        require_device_ptr(a, op, "a");
-        require_device_ptr(a_scales, op, "a_scales");
-        require_device_ptr(b, op, "b");
-        require_device_ptr(b_scales, op, "b_scales");
+        if (k > 0) {   // matrices without columns have no address
+            require_device_ptr(a, op, "a");
+            require_device_ptr(a_scales, op, "a_scales");
+            require_device_ptr(b, op, "b");
+            require_device_ptr(b_scales, op, "b_scales");
+        }
         optional_device_ptr(bias, op, "bias");
         require_device_ptr(out, op, "out");
         require(aligned(a, 16) && aligned(b, 16), "gemm_fp8: a and b must be 16-byte aligned");
@@ -429,6 +431,7 @@ WindowShape window_shape(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
     require(batch < kSizeLimit && heads < kSizeLimit && q_len < kSizeLimit && kv_len < kSizeLimit &&
                 heads / kv_heads * q_len < kSizeLimit,
             "attention_window: kv_len and heads * q_len must be below 2^30");
+    require(batch * heads < (int64_t{1} << 31), "attention_window: batch * heads must be below 2^31");
     auto side = [](int64_t w) { return w < 0 ? -1 : static_cast<int>(std::min(w, kSizeLimit)); };
     return WindowShape{batch, heads, kv_heads, q_len, kv_len, head_dim, 0, 0, 0, 0.f, side(left), side(right),
                        static_cast<int>(std::min(sinks, kSizeLimit))};

@@ -638,7 +638,9 @@ void launch_attention_window(const bf16_t* q, const bf16_t* k, const bf16_t* v, 
     a.splits = how.splits;
     const int64_t grid = tiles * sh.batch * sh.kv_heads * how.splits;
     require(grid < (int64_t{1} << 31), "attention_window: too many queries");
-    ProfileScope ps(sh.q_len == sh.kv_len ? K_ATTN_SELF : K_ATTN_CROSS, s, 0);
+    // the operations of windows that lie inside the sequence; the lengths themselves are on the device
+    const int64_t seen = sh.left < 0 || sh.right < 0 ? sh.kv_len : std::min(sh.kv_len, int64_t{sh.left} + sh.right + 1 + sh.sinks);
+    ProfileScope ps(sh.q_len == sh.kv_len ? K_ATTN_SELF : K_ATTN_CROSS, s, 4.0 * sh.batch * sh.heads * sh.q_len * seen * sh.head_dim);
     const int dt = (a.D + 15) / 16;
     if (dt <= 2) launch<2>(a, how, grid, s);
     else if (dt <= 4) launch<4>(a, how, grid, s);

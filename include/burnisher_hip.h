@@ -230,7 +230,7 @@ int64_t bh_gemm_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k);
  * Element (b, s, h, d) of q lives at q[(b * q_len + s) * ld_q + h * head_dim + d], of k and v at
  * [(b * kv_len + s) * ld_kv + h * head_dim + d] and of out with ld_out. head_dim is a multiple of 8
  * up to 128, the row strides are multiples of 8 (ld_out of 4), q, k and v 16-byte and out 8-byte
- * aligned, kv_len and heads * q_len below 2^30 and ld_kv below 2^24.
+ * aligned, kv_len and heads * q_len below 2^30, batch * heads below 2^31 and ld_kv below 2^24.
  * It has no counterpart in the reference. `workspace` as in bh_gemm_fp8: the partial results of keys
  * split over workgroups (few queries, many keys). */
 int bh_attention_window(const void* q, int64_t ld_q, const void* k, const void* v, int64_t ld_kv,

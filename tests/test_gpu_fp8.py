@@ -250,6 +250,41 @@ def test_gemm_of_an_empty_sum_is_the_epilogue_of_the_bias(hip):
         assert torch.equal(got, bias.expand(m, 5))
 
 
+def test_gemm_of_matrices_without_columns_takes_no_addresses(hip):
+    import torch
+    import burnisher_amd as bh
+    bias = normal((5,), 1, torch.float32)
+    for m in (3, 200):
+        out = torch.full((m, 5), 9.0, device="cuda")
+        bh.call("bh_gemm_fp8", None, None, None, None, bias.data_ptr(), out.data_ptr(), m, 5, 0, 0, F32, None, 0,
+                bh.stream_ptr())
+        assert torch.equal(out, bias.expand(m, 5))
+
+
+def test_gemm_stays_inside_its_workspace_and_refuses_a_small_one(hip):
+    import torch
+    import burnisher_amd as bh
+    m, n, k = 600, 256, 8192
+    need = bh.lib().bh_gemm_fp8_workspace_bytes(m, n, k)
+    assert need > 0
+    a, sa, b, sb = operands(m, n, k, 1)
+    out = torch.zeros(m, n, dtype=torch.bfloat16, device="cuda")
+    ws = torch.full((need + 4096,), 0x5a, dtype=torch.uint8, device="cuda")
+
+    def call(at, size):
+        return bh.lib().bh_gemm_fp8(a.data_ptr(), sa.data_ptr(), b.data_ptr(), sb.data_ptr(), None, out.data_ptr(), m, n,
+                                    k, 0, BF16, at, size, bh.stream_ptr())
+
+    used = 4 * m * n * 2   # at least two slices
+    assert call(ws.data_ptr(), used // 2) != 0 and b"this call needs" in bh.lib().bh_last_error()
+    assert call(ws.data_ptr() + 8, need) != 0 and b"16-byte" in bh.lib().bh_last_error()
+    torch.cuda.synchronize()
+    assert not out.any() and (ws == 0x5a).all(), "a refused call wrote"
+    assert call(ws.data_ptr(), need) == 0
+    assert (ws[need:] == 0x5a).all(), "written past the workspace"
+    assert torch.equal(out, run_gemm(a, sa, b, sb, None, k))
+
+
 def test_gemm_small_whole_numbers_are_exact(hip):
     # integers up to 8 with power-of-two scales: every product and sum is exact in either instruction
     import torch

@@ -261,6 +261,30 @@ def test_offsets_beyond_32_bits(hip):
     compare(got, q, short, short, None, None, -1, 0, 0)
 
 
+def test_stays_inside_its_workspace_and_refuses_a_small_one(hip):
+    import torch
+    import burnisher_amd as bh
+    batch, heads, kvh, kv_len, d = 1, 8, 2, 6000, 64
+    q, k, v = normal((batch, 1, heads, d), 1), normal((batch, kv_len, kvh, d), 2), normal((batch, kv_len, kvh, d), 3)
+    need = bh.lib().bh_attention_window_workspace_bytes(batch, heads, kvh, 1, kv_len, d, -1, 0, 0)
+    assert need > 0
+    out = torch.zeros_like(q)
+    ws = torch.full((need + 4096,), 0x5a, dtype=torch.uint8, device="cuda")
+
+    def call(at, size):
+        return bh.lib().bh_attention_window(q.data_ptr(), heads * d, k.data_ptr(), v.data_ptr(), kvh * d, out.data_ptr(),
+                                            heads * d, batch, heads, kvh, 1, kv_len, d, 0.0, -1, 0, 0, None, None, BF16,
+                                            at, size, bh.stream_ptr())
+
+    assert call(ws.data_ptr(), need - 1) != 0 and b"this call needs" in bh.lib().bh_last_error()
+    assert call(ws.data_ptr() + 4, need) != 0 and b"16-byte" in bh.lib().bh_last_error()
+    torch.cuda.synchronize()
+    assert not out.any() and (ws == 0x5a).all(), "a refused call wrote"
+    assert call(ws.data_ptr(), need) == 0
+    assert (ws[need:] == 0x5a).all(), "written past the workspace"
+    assert torch.equal(out, run(q, k, v, None, None, -1, 0, 0))
+
+
 def test_in_a_graph_and_on_two_streams(hip):
     import torch
     import burnisher_amd as bh

@@ -83,6 +83,8 @@ def test_workspace_queries_refuse_and_answer():
     lib = bh.lib()
     assert lib.bh_gemm_fp8_workspace_bytes(-1, 4, 4) == -1 and b"negative" in lib.bh_last_error()
     assert lib.bh_attention_window_workspace_bytes(1, 8, 3, 1, 64, 64, -1, 0, 0) == -1
+    assert lib.bh_attention_window_workspace_bytes(1 << 24, 1 << 24, 1 << 24, 1, 64, 64, -1, 0, 0) == -1
+    assert b"batch * heads" in lib.bh_last_error()
     assert lib.bh_gemm_fp8_workspace_bytes(0, 4, 4) == 0 and lib.bh_last_error() == b""
     assert lib.bh_attention_window_workspace_bytes(0, 8, 2, 1, 64, 64, -1, 0, 0) == 0
 
