@@ -225,6 +225,31 @@ def test_gemm_tiles(hip, m, n, k, dtype):
     check_gemm(m, n, k, dtype=dtype, with_bias=k % 2 == 1)
 
 
+# rows of out that start on lines of 128 bytes and rows that do not, tiles inside and across the edge
+ROW_SIZES = [(195, 4360, 272), (235, 4288, 272), (131, 280, 4005), (141, 256, 5008), (2816, 1416, 256), (1697, 2432, 256),
+             (266, 3904, 3968), (1836, 4160, 384), (2736, 2200, 256), (2304, 3592, 256), (2495, 3264, 256), (2736, 4424, 256),
+             (2816, 4608, 256), (2637, 2952, 256), (515, 3588, 4224), (1318, 4420, 256), (385, 4160, 3749), (2927, 2820, 256)]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("m,n,k", ROW_SIZES)
+def test_gemm_output_rows_of_any_alignment(hip, m, n, k, dtype):
+    import torch
+    import burnisher_amd as bh
+    got = check_gemm(m, n, k, act=2, with_bias=True, dtype=dtype)
+    a, sa, b, sb = operands(m, n, k, m * 7 + n * 3 + k)
+    bias = normal((n,), 3, getattr(torch, dtype))
+    need = max(16, bh.lib().bh_gemm_fp8_workspace_bytes(m, n, k))
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    for shift in (16 // got.element_size(), 1):
+        buf = torch.full((m * n + 64,), -3.0, dtype=got.dtype, device="cuda")
+        out = buf[shift:shift + m * n]
+        bh.call("bh_gemm_fp8", a.data_ptr(), sa.data_ptr(), b.data_ptr(), sb.data_ptr(), bias.data_ptr(), out.data_ptr(), m,
+                n, k, 2, BF16 if dtype == "bfloat16" else F32, ws.data_ptr(), need, bh.stream_ptr())
+        assert torch.equal(out.view(m, n), got)
+        assert (buf[:shift] == -3.0).all() and (buf[shift + m * n:] == -3.0).all(), "written outside"
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("act", [0, 1, 2])
 @pytest.mark.parametrize("m,n,k", [(1, 300, 400), (40, 129, 256), (333, 640, 520), (2048, 256, 128)])
