@@ -395,3 +395,13 @@ def test_quantized_projection_of_a_wide_activation(hip):
     small = 2.0 ** -10 / 448 * (x.double().abs().amax(1)[:, None] * w.double().abs().sum(1) +
                                 w.double().abs().amax() * x.double().abs().sum(1)[:, None])
     assert ((got - want).abs() <= (2 * 2.0 ** -4 + 2.0 ** -7) * size + 2 * small + 2.0 ** -8 * want.abs()).all()
+
+
+def test_the_default_stream_is_the_current_one(hip):
+    import torch
+    import burnisher_amd as bh
+    other = torch.cuda.Stream()
+    assert bh.stream_ptr() == torch.cuda.current_stream().cuda_stream
+    assert bh.stream_ptr(other) == other.cuda_stream
+    with torch.cuda.stream(other):
+        assert bh.stream_ptr() == other.cuda_stream
