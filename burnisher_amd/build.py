@@ -51,7 +51,7 @@ def sources() -> list[Path]:
 # copies all 80 of them between the register files), and it is compiled without IEEE NaN rules
 # so a maximum over MFMA results is one v_max3 per two inputs, not a quieting v_max per input.
 # flash512.hip keeps its scores in VGPRs the same way (its output sums are accumulation registers,
-# by hand).
+# by hand). So does gemm_fp8.hip: every block's sum passes from the matrix cores to a vector multiply-add.
 # cross_fused.hip runs the same attention code after its projection, so it takes the same options.
 # denoise.hip evaluates the guidance combine and the solver update in fp64 exactly as the
 # reference's x86-64 build does, which forms no multiply-add. elementwise.hip holds the kernels

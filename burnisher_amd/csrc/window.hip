@@ -263,9 +263,13 @@ __device__ __forceinline__ bool sees_all(int base, int end, int lo1, int hi0, in
 // ---- many rows: 128 a workgroup, 32 a wave; K and V in blocks of 64 keys that its four waves share --------
 //
 // Two workgroups a CU, each with two slots in LDS for K and for V; deeper rings, tiles of 256 rows and 32 x 32 x 16
-// products were no faster. What bounds it: the vector instructions, 32 exponentials (16 cycles each) and about 90 others
+// products were no faster. What bounds it: the vector instructions, 32 exponentials (16 cycles each) and about 75 others
 // a lane and block, run beside the matrix ones only in part (2 x 16384 tokens of 16 heads, window 1024 to either side,
-// head_dim 64: vector 67%, matrix 38% of the time; head_dim 128: 46% and 46%).
+// head_dim 64: vector 67%, matrix 38% of the time; head_dim 128: 46% and 46%). Without the exponentials the same calls
+// take 15% and 8% less, without the running maximum 18% and 6%; finding the maximum among the output product's matrix
+// instructions, or acting on it behind the barrier, gained nothing. Measured there: 390 us at head_dim 64 (680 TFLOP/s),
+// 465 to 485 at 72 (whose columns are computed as 80 and 96), 590 at 128; 2 x 4096 tokens of 32 / 8 heads of 128, window
+// 1023 back, 167 to 183 us.
 
 constexpr int kKeys = 64, kManyRows = 128;
 
@@ -391,7 +395,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_window_many(WindowArgs a) {
 // ---- few rows: 16 QT a workgroup, whose waves take pieces of 32 keys in turn, each through LDS of its own ----
 //
 // Bound by the keys' bytes: a wave waits only for its own loads, two pieces in flight, and the waves' sums meet
-// at the end. With `splits` the keys go to several workgroups, whose partial results k_window_join sums.
+// at the end. With `splits` the keys go to several workgroups, whose partial results k_window_join sums (4.8 us for
+// 512 rows of 128 in two splits: a launch). 16 sequences of one token, 32 / 8 heads of 128, window 4095 back in up
+// to 8192 keys: 54 us with the join, 5.0 TB/s.
 
 constexpr int kPiece = 32;
 
