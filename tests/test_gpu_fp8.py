@@ -379,6 +379,41 @@ def test_gemm_in_a_graph_and_on_two_streams(hip, m, n, k):
         assert torch.equal(out[0], run_gemm(*sets[0], None, k)), "a replay differs from the call"
 
 
+def within(got, want_tol):
+    want, tol = want_tol
+    return ((got.double() - want).abs() <= tol).all()
+
+
+def test_matrices_beyond_32_bits(hip):
+    import torch
+    import burnisher_amd as bh
+    # 530432 rows of 8192: 8.7 GB of bf16, 4.3 GB of codes, as the activations and as the weights of a product
+    rows, k, tail = 1024 * 518, 8192, 300
+    piece = normal((1024, k), 1, torch.bfloat16)
+    x = piece.repeat(518, 1)
+    small, small_s = quantize_plain(normal((40, k), 2, torch.float32, 0.02), 128)
+    q, sq = quantize(x, 1)
+    want, want_s = quantize_plain(piece, 1)
+    for at in (0, rows - 1024):
+        assert same_bits(q[at:at + 1024], want) and torch.equal(sq[:, at:at + 1024], want_s)
+    out = run_gemm(q, sq, small, small_s, None, k)
+    assert within(out[-tail:], gemm_plain(q[-tail:], sq[:, -tail:].contiguous(), small, small_s, None, k, 0, "bfloat16"))
+    q, sq = quantize(x, 128)
+    want, want_s = quantize_plain(piece, 128)
+    for at in (0, rows - 1024):
+        assert same_bits(q[at:at + 1024], want) and torch.equal(sq[at // 128:at // 128 + 8], want_s)
+    few, few_s = quantize_plain(normal((3, k), 3, torch.float32), 1)
+    out = run_gemm(few, few_s, q, sq, None, k)
+    assert within(out[:, -384:], gemm_plain(few, few_s, q[-384:], sq[-3:], None, k, 0, "bfloat16"))
+    del x, q, out
+    # 4.6 GB of output
+    m, n, k = 70000, 33000, 130
+    a, sa, b, sb = operands(m, n, k, 4)
+    out = run_gemm(a, sa, b, sb, None, k)
+    assert within(out[-200:], gemm_plain(a[-200:], sa[:, -200:].contiguous(), b, sb, None, k, 0, "bfloat16"))
+    bh.check(0)
+
+
 def test_quantized_projection_of_a_wide_activation(hip):
     # as a program uses them: weights quantised once, activations per call, the product against the
     # unquantised one; an e4m3 rounding is at most 2^-4 of a value, so the error of a sum of K products of two
