@@ -191,17 +191,19 @@ struct Geom {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 // gk::dma16 with a uniform base and a 32-bit offset a lane; dma4 moves four bytes a lane.
+// The wait states: one behind m0, five behind a vector instruction that wrote `base` (a register brought back from
+// where the compiler had put it), which it does not count for inline assembly.
 __device__ __forceinline__ uint32_t lds_address(const char* p) {
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(p)));
 }
 __device__ __forceinline__ void dma16_at(const void* base, uint32_t off, const char* lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
                  :
                  : "s"(lds_address(lds)), "v"(off), "s"(base)
                  : "memory", "m0");
 }
 __device__ __forceinline__ void dma4_at(const void* base, uint32_t off, const char* lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2"
                  :
                  : "s"(lds_address(lds)), "v"(off), "s"(base)
                  : "memory", "m0");

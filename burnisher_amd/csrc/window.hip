@@ -67,8 +67,10 @@ __device__ __forceinline__ uint32_t lds_address(const char* p) {
 #pragma clang diagnostic ignored "-Winline-asm"
 // Lane L's 16 bytes at base + off land at LDS address lds + 16 L (`base` and `lds` uniform). Inline assembly so
 // that the compiler does not wait for these loads by itself: s_waitcnt below covers them.
+// The wait states: one behind m0, five behind a vector instruction that wrote `base` (a register brought back from
+// where the compiler had put it), which it does not count for inline assembly.
 __device__ __forceinline__ void dma16(const void* base, uint32_t off, const char* lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
                  :
                  : "s"(lds_address(lds)), "v"(off), "s"(base)
                  : "memory", "m0");
@@ -262,14 +264,15 @@ __device__ __forceinline__ bool sees_all(int base, int end, int lo1, int hi0, in
 
 // ---- many rows: 128 a workgroup, 32 a wave; K and V in blocks of 64 keys that its four waves share --------
 //
-// Two workgroups a CU, each with two slots in LDS for K and for V; deeper rings, tiles of 256 rows and 32 x 32 x 16
-// products were no faster. What bounds it: the vector instructions, 32 exponentials (16 cycles each) and about 75 others
-// a lane and block, run beside the matrix ones only in part (2 x 16384 tokens of 16 heads, window 1024 to either side,
-// head_dim 64: vector 67%, matrix 38% of the time; head_dim 128: 46% and 46%). Without the exponentials the same calls
-// take 15% and 8% less, without the running maximum 18% and 6%; finding the maximum among the output product's matrix
-// instructions, or acting on it behind the barrier, gained nothing. Measured there: 390 us at head_dim 64 (680 TFLOP/s),
-// 465 to 485 at 72 (whose columns are computed as 80 and 96), 590 at 128; 2 x 4096 tokens of 32 / 8 heads of 128, window
-// 1023 back, 167 to 183 us.
+// Two workgroups a CU (three up to head_dim 64), each with two slots in LDS for K and for V; deeper rings, tiles of 256
+// rows and 32 x 32 x 16 products were no faster. What bounds it: the vector instructions, 32 exponentials and about 75
+// others a lane and block, run beside the matrix ones only in part, and a block's loads wait for each other while they are
+// issued (600 of 3200 to 4500 cycles; put between the products they cost more registers than that). Without the
+// exponentials a call takes 8 to 15% less; finding the maximum among the output product's matrix instructions, or acting on
+// it behind the barrier, gained nothing. Which blocks a wave sees, and sees whole, are ranges found before the loop, and
+// whole blocks load without a branch a load: at head_dim 64 388 -> 340 us. Measured (2 x 16384 tokens of 16 heads, window
+// 1024 to either side): head_dim 64 340 us (780 TFLOP/s), 72 450 (its columns are computed as 80 and 96), 128 571 (930);
+// 2 x 4096 tokens of 32 / 8 heads of 128, window 1023 back, 163 to 178; 2 x 300 of 64 heads of 64, 128 either side, 15.
 
 constexpr int kKeys = 64, kManyRows = 128;
 
@@ -277,7 +280,7 @@ template <int DT>
 __global__ void __launch_bounds__(kThreads, 2) k_window_many(WindowArgs a) {
     constexpr int QT = 2, kChunks = DT * 2, KP = k_pitch(kChunks), VP = v_pitch(kChunks);   // for the widest head_dim here
     constexpr int kKBytes = kKeys * 16 * KP, kVBytes = kKeys * 16 * VP;
-    constexpr int kKItems = (KP + 3) / 4, kVItems = (VP + 3) / 4;   // loads a wave issues per block, at most
+    constexpr int kItems = (KP + VP + 3) / 4;   // loads a wave issues per block, at most
     __shared__ __attribute__((aligned(1024))) char kmem[2 * kKBytes], vmem[2 * kVBytes];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int T = a.tiles * a.B * a.KH;
@@ -298,28 +301,55 @@ __global__ void __launch_bounds__(kThreads, 2) k_window_many(WindowArgs a) {
     const uint32_t ld_bytes = static_cast<uint32_t>(a.ld_kv) * 2;
     const int chunks = a.D / 8;
     const int64_t first = static_cast<int64_t>(b) * a.Skv * a.ld_kv + static_cast<int64_t>(kh) * a.D;
-    // a wave's loads of a block: rows 4 i + wave of 1 KiB of its LDS image
-    uint32_t koff[kKItems], voff[kVItems];
+    // A block's loads are the KP rows of 1 KiB of K's LDS image and then V's VP: row 4 i + wave is wave's i-th, the last
+    // one of some waves only. K of one block goes with V of the block before it.
+    uint32_t off[kItems];
 #pragma unroll
-    for (int i = 0; i < kKItems; ++i) koff[i] = chunk_offset<KP>(i * 4 + wave, lane, chunks, kKeys - 1, ld_bytes);
+    for (int i = 0; i < kItems; ++i) {
+        const int n = i * 4 + wave;
+        off[i] = n < KP ? chunk_offset<KP>(n, lane, chunks, kKeys - 1, ld_bytes) : chunk_offset<VP>(n - KP, lane, chunks, kKeys - 1, ld_bytes);
+    }
+    uint32_t off_last[kItems - KP / 4];   // V's of the last block, which ends inside it in most calls
 #pragma unroll
-    for (int i = 0; i < kVItems; ++i) voff[i] = chunk_offset<VP>(i * 4 + wave, lane, chunks, kKeys - 1, ld_bytes);
-    auto load_k = [&](int j) {
-        const int base = blocks.base(j), last = blocks.end(j) - base - 1;
-        const bf16_t* k = a.k + first + static_cast<int64_t>(base) * a.ld_kv;
+    for (int i = KP / 4; i < kItems; ++i) {
+        const int last = blocks.n > 0 ? blocks.end(blocks.n - 1) - blocks.base(blocks.n - 1) - 1 : 0;
+        off_last[i - KP / 4] = chunk_offset<VP>(max(i * 4 + wave - KP, 0), lane, chunks, min(last, kKeys - 1), ld_bytes);
+    }
+    const bf16_t *k0 = a.k + first, *v0 = a.v + first;
+    auto key_offset = [&](int base) { return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(base)) * ld_bytes / 2); };
+    // K of block jk and V of block jv (jv < 0: not), where there are such blocks. Keys past a block's end: K's are masked, so
+    // they may be read where there is memory; V's are the last one again.
+    auto load = [&](int jk, int jv) {
+        const int kb = blocks.base(jk), vb = blocks.base(max(jv, 0)), k_last = blocks.end(jk) - kb - 1, v_last = blocks.end(max(jv, 0)) - vb - 1;
+        const bf16_t *k = k0 + key_offset(kb), *v = v0 + key_offset(vb);
+        const char *kl = kmem + (jk & 1) * kKBytes, *vl = vmem + (jv & 1) * kVBytes - KP * 1024;
+        const bool with_k = jk < blocks.n, with_v = (jv >= 0) & (jv < blocks.n), k_whole = kb + kKeys <= a.Skv;
+        if (with_k & with_v & k_whole & (v_last >= kKeys - 1)) {
 #pragma unroll
-        for (int i = 0; i < kKItems; ++i) {
-            const int n = i * 4 + wave;
-            if (n < KP) dma16(k, last < kKeys - 1 ? chunk_offset<KP>(n, lane, chunks, last, ld_bytes) : koff[i], kmem + (j & 1) * kKBytes + n * 1024);
+            for (int i = 0; i < kItems; ++i) {
+                const int n = i * 4 + wave;
+                if (i * 4 + 3 < KP + VP || n < KP + VP) dma16(n < KP ? k : v, off[i], (n < KP ? kl : vl) + n * 1024);
+            }
+            return;
         }
-    };
-    auto load_v = [&](int j) {
-        const int base = blocks.base(j), last = blocks.end(j) - base - 1;
-        const bf16_t* v = a.v + first + static_cast<int64_t>(base) * a.ld_kv;
+        if ((jv < 0) & k_whole) {
 #pragma unroll
-        for (int i = 0; i < kVItems; ++i) {
-            const int n = i * 4 + wave;
-            if (n < VP) dma16(v, last < kKeys - 1 ? chunk_offset<VP>(n, lane, chunks, last, ld_bytes) : voff[i], vmem + (j & 1) * kVBytes + n * 1024);
+            for (int i = 0; i * 4 < KP; ++i)
+                if (i * 4 + wave < KP) dma16(k, off[i], kl + (i * 4 + wave) * 1024);
+            return;
+        }
+        if (!with_k & (jv == blocks.n - 1)) {
+#pragma unroll
+            for (int i = KP / 4; i < kItems; ++i) {
+                const int n = i * 4 + wave;
+                if (n >= KP && n < KP + VP) dma16(v, off_last[i - KP / 4], vl + n * 1024);
+            }
+            return;
+        }
+#pragma unroll 1
+        for (int n = with_k ? wave : KP + (wave + 3 * KP) % 4; n < (with_v ? KP + VP : KP); n += 4) {
+            if (n < KP) dma16(k, chunk_offset<KP>(n, lane, chunks, min(k_last, kKeys - 1), ld_bytes), kl + n * 1024);
+            else dma16(v, chunk_offset<VP>(n - KP, lane, chunks, min(v_last, kKeys - 1), ld_bytes), vl + n * 1024);
         }
     };
     auto join = [&]() {   // this wave's loads have landed and its reads are done; behind the barrier everyone's
@@ -330,21 +360,22 @@ __global__ void __launch_bounds__(kThreads, 2) k_window_many(WindowArgs a) {
     };
     f32x4_t s[4][QT];
     float mx[QT];
-    auto seen = [&](int j) {   // some row of the wave sees some key of the block
-        const int base = blocks.base(j);
-        return j < blocks.n && base < min(blocks.end(j), hi1) && (base + kKeys > lo0 || base < a.sinks);
-    };
+    // The wave's blocks, as ranges of their numbers: those of which some row sees some key, and those of which every row
+    // sees every key (at least those that the ranges hold), before the window and in it.
+    const int lo = blocks.lo, hi = blocks.hi, nb1 = blocks.nb1;
+    const int seen_near = (min(blocks.near, hi1) + kKeys - 1) / kKeys, whole_near = min(blocks.near, hi0) / kKeys;
+    const int seen0 = nb1 + (a.sinks > lo ? 0 : max(lo0 - lo, 0) / kKeys), seen1 = nb1 + (max(min(hi, hi1) - lo, 0) + kKeys - 1) / kKeys;
+    const int whole0 = nb1 + (max(lo1 - lo, 0) + kKeys - 1) / kKeys, whole1 = nb1 + max(min(hi, hi0) - lo, 0) / kKeys;
+    auto seen = [&](int j) { return (j < seen_near) | ((j >= seen0) & (j < seen1)); };
     auto maximum = [&](int j) {
-        const int base = blocks.base(j), end = blocks.end(j);
-        if (!sees_all<kKeys>(base, end, lo1, hi0, a.sinks)) w.template mask<4>(s, base, end, a.sinks, lane);
+        if (!((j < whole_near) | ((j >= whole0) & (j < whole1)))) w.template mask<4>(s, blocks.base(j), blocks.end(j), a.sinks, lane);
         w.template largest<4>(mx, s, a.c);
         w.raise(mx);
     };
     if (blocks.n > 0) {
-        load_k(0);
-        load_v(0);
+        load(0, -1);
         join();
-        if (blocks.n > 1) load_k(1);
+        load(1, 0);
 #pragma unroll
         for (int t = 0; t < 4; ++t) w.scores(s[t], t, kmem, KP * 16, a.D, lane);
         maximum(0);
@@ -354,9 +385,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_window_many(WindowArgs a) {
     // have been read. Scores that no row of the wave sees are -inf here, so a block that it does not see adds nothing.
     for (int j = 0; j < blocks.n; ++j) {
         join();
-        if (j + 2 < blocks.n) load_k(j + 2);
-        if (j + 1 < blocks.n) load_v(j + 1);
-        if (!seen(j) && !seen(j + 1)) continue;
+        load(j + 2, j + 1);
+        if (!(seen(j) | seen(j + 1))) continue;
         const char* kp = kmem + ((j + 1) & 1) * kKBytes;   // behind the last block: scores that nobody uses
         u32x2_t half[4][QT];
         bf16x8_t p[2][QT];
