@@ -464,13 +464,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_window_few(WindowArgs a) {
     auto load = [&](int j, int slot) {
         const int base = pieces.base(j), last = pieces.end(j) - base - 1;
         const bf16_t *k = a.k + first + static_cast<int64_t>(base) * a.ld_kv, *v = a.v + first + static_cast<int64_t>(base) * a.ld_kv;
+        char* to = own + slot * kStage;
+        if (last >= kPiece - 1) {
 #pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-            uint32_t o = off[i];
-            if (last < kPiece - 1)
-                o = i < kK ? chunk_offset<KP>(i, lane, chunks, last, ld_bytes) : chunk_offset<VP>(i - kK, lane, chunks, last, ld_bytes);
-            dma16(i < kK ? k : v, o, own + slot * kStage + i * 1024);
+            for (int i = 0; i < kItems; ++i) dma16(i < kK ? k : v, off[i], to + i * 1024);
+            return;
         }
+#pragma unroll 1
+        for (int i = 0; i < kItems; ++i)
+            dma16(i < kK ? k : v, i < kK ? chunk_offset<KP>(i, lane, chunks, last, ld_bytes) : chunk_offset<VP>(i - kK, lane, chunks, last, ld_bytes),
+                  to + i * 1024);
     };
     if (j0 < j1) load(j0, 0);
     w.init(a, keys, b, kh, row0, rows, lane);
@@ -599,7 +602,7 @@ int device_cus() {
 //    5.2 TB/s (a quarter more on fewer workgroups than CUs);
 //  - a join costs 3 + 0.25 a split and its partial results at 3 TB/s.
 // 16 sequences of a token each, 32 / 8 heads of 128, 4096 keys: two splits 57 us, none 65, k_window_many 90. Four times
-// 64 tokens of the same: 32-row tiles 54, 16-row 82, 64-row 80, k_window_many 97. 2 x 64 heads of 300 tokens, head_dim 64:
+// 64 tokens of the same: 32-row tiles 52, 16-row 82, 64-row 80, k_window_many 97. 2 x 64 heads of 300 tokens, head_dim 64:
 // k_window_many 15.6, 32-row tiles 24.
 struct Plan {
     int few;      // 0: k_window_many
