@@ -367,13 +367,15 @@ __device__ __forceinline__ float act_out(float v, int act) {
 
 // Eight values of the bias from column n, -0.0 (which adds nothing to any value) without one and past the end.
 template <typename OUT>
-__device__ __forceinline__ void load_bias(const OUT* bias, int64_t n, int64_t N, bool vec, float (&b)[8]) {
-    if (bias && vec && n + 8 <= N) {
+__device__ __forceinline__ void load_bias(const OUT* bias, int64_t n, int64_t N, float (&b)[8]) {
+    if (bias && n + 8 <= N) {
         if constexpr (sizeof(OUT) == 4) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) b[e] = bias[n + e];
         } else {
-            gk::unpack8(*reinterpret_cast<const uint4*>(bias + n), b);
+            typedef u32x4_t Any __attribute__((aligned(2)));
+            const u32x4_t w = *reinterpret_cast<const Any*>(bias + n);
+            gk::unpack8(make_uint4(w[0], w[1], w[2], w[3]), b);
         }
         return;
     }
@@ -386,13 +388,15 @@ __device__ __forceinline__ uint32_t swap_pair(uint32_t v) {
     return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xb1, 0xf, 0xf, true));   // quad_perm 1 0 3 2
 }
 
+// 16 bytes of a row that starts anywhere: memory takes them at the alignment of an element (8192 x 8191 x 1152 135 us, element by element 209).
 template <bool LINES, typename V, typename T>
 __device__ __forceinline__ void store16(V v, T* p) {
+    typedef V Any __attribute__((aligned(sizeof(T))));
     if constexpr (LINES) __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
-    else *reinterpret_cast<V*>(p) = v;
+    else *reinterpret_cast<Any*>(p) = v;
 }
 
-// A tile that lies inside an output of 16-byte aligned rows. Lanes lr and lr ^ 1 exchange halves, so that eight lanes
+// A tile that lies inside the output. Lanes lr and lr ^ 1 exchange halves, so that eight lanes
 // write 128 consecutive bytes of a row. LINES: those are whole lines, which go past the caches (8192 x 8192 x 1152:
 // 107 -> 94 us). Parts of lines are left for L2 to put together (8192 x 4616 x 1152 68 us, past the caches 75).
 template <int MT, int NP, typename OUT, bool LINES>
@@ -455,19 +459,18 @@ __device__ __forceinline__ void store_inside(const f32x4_t (&acc)[MT][2 * NP], c
     }
 }
 
-// A lane's 8 consecutive columns of MT rows a column pair. `vec`: rows of out and the bias are 16-byte aligned.
-// The bias is read before the first store: vmcnt counts loads and stores in order, so a load behind a store
+// A lane's 8 consecutive columns of MT rows a column pair. The bias is read before the first store: vmcnt counts loads and stores in order, so a load behind a store
 // waits until memory has taken that.
 template <int MT, int NP, typename OUT>
-__device__ __forceinline__ void store(const f32x4_t (&acc)[MT][2 * NP], const Fp8Args& p, bool vec, int64_t m0, int64_t n0,
+__device__ __forceinline__ void store(const f32x4_t (&acc)[MT][2 * NP], const Fp8Args& p, int64_t m0, int64_t n0,
                                       int wm, int wn, int lr, int hi) {
     OUT* out = static_cast<OUT*>(p.out);
     const int64_t m = m0 + wm * 16 * MT + lr * MT;
     float b[NP][8];
 #pragma unroll
     for (int q = 0; q < NP; ++q)
-        load_bias(static_cast<const OUT*>(p.bias), n0 + (wn * NP + q) * 32 + hi * 8, p.n, vec, b[q]);
-    if (vec && m0 + 64 * MT <= p.m && n0 + 64 * NP <= p.n) {   // uniform: the whole tile
+        load_bias(static_cast<const OUT*>(p.bias), n0 + (wn * NP + q) * 32 + hi * 8, p.n, b[q]);
+    if (m0 + 64 * MT <= p.m && n0 + 64 * NP <= p.n) {   // uniform: the whole tile
         if (((reinterpret_cast<uintptr_t>(out) | p.n * sizeof(OUT)) & 127) == 0) {
             asm volatile("");   // here and behind, or the two calls become one of ordinary stores
             store_inside<MT, NP, OUT, true>(acc, b, out, p.n, p.act, m0, n0, wm, wn, lr, hi);
@@ -489,12 +492,13 @@ __device__ __forceinline__ void store(const f32x4_t (&acc)[MT][2 * NP], const Fp
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = act_out<OUT>(acc[i][2 * q + (e >> 2)][e & 3] + b[q][e], p.act);
             OUT* dst = out + (m + i) * p.n + n;
-            if (vec && whole) {
+            if (whole) {
                 if constexpr (sizeof(OUT) == 4) {
-                    *reinterpret_cast<f32x4_t*>(dst) = f32x4_t{v[0], v[1], v[2], v[3]};
-                    *reinterpret_cast<f32x4_t*>(dst + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+                    store16<false>(f32x4_t{v[0], v[1], v[2], v[3]}, dst);
+                    store16<false>(f32x4_t{v[4], v[5], v[6], v[7]}, dst + 4);
                 } else {
-                    *reinterpret_cast<uint4*>(dst) = gk::pack8(v);
+                    const uint4 w = gk::pack8(v);
+                    store16<false>(u32x4_t{w.x, w.y, w.z, w.w}, dst);
                 }
             } else {
 #pragma unroll
@@ -510,8 +514,7 @@ template <int MT, int NP>
 __device__ __forceinline__ void store_partial(const f32x4_t (&acc)[MT][2 * NP], const Fp8Args& p, int slice, int64_t m0,
                                               int64_t n0, int wm, int wn, int lr, int hi) {
     float* part = p.part + slice * p.m * p.n;
-    const bool vec = p.n % 4 == 0;
-    if (vec && m0 + 64 * MT <= p.m && n0 + 64 * NP <= p.n) {
+    if (m0 + 64 * MT <= p.m && n0 + 64 * NP <= p.n) {
         float b[NP][8];
 #pragma unroll
         for (int q = 0; q < NP; ++q)
@@ -530,8 +533,8 @@ __device__ __forceinline__ void store_partial(const f32x4_t (&acc)[MT][2 * NP], 
             for (int i = 0; i < MT; ++i) {
                 if (m + i >= p.m || n >= p.n) continue;
                 float* dst = part + (m + i) * p.n + n;
-                if (vec) {
-                    *reinterpret_cast<f32x4_t*>(dst) = acc[i][2 * q + h];
+                if (n + 4 <= p.n) {
+                    store16<false>(acc[i][2 * q + h], dst);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
@@ -556,8 +559,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm_fp8_tile(Fp8Args p, int ti
     const int kb1 = static_cast<int>(static_cast<int64_t>(slice + 1) * p.blocks / slices);   // this slice's blocks of K
     const int KT = kb1 - kb0, grid = static_cast<int>(gridDim.x), tiles = tiles_m * tiles_n;
     const int total = (tiles - static_cast<int>(blockIdx.x) + grid - 1) / grid * KT;
-    const bool vec = (p.n * static_cast<int64_t>(sizeof(OUT))) % 16 == 0 &&
-                     ((reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.bias)) & 15) == 0;
     // Rows that end inside a block of K: the chunks of 16 that the last block has, and for a lane whose chunk lies
     // past them the distance back to the block's first chunk, which it loads instead (multiply() takes it as zero).
     const int last = static_cast<int>((p.ld - 1) / 16 % 8) + 1;
@@ -654,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm_fp8_tile(Fp8Args p, int ti
             int64_t m0, n0;
             tile_at<MT, NP>(tile, tiles_m, tiles_n, group_m, m0, n0);
             if (slices > 1) store_partial<MT, NP>(acc, p, slice, m0, n0, wm, wn, lr, hi);
-            else store<MT, NP, OUT>(acc, p, vec, m0, n0, wm, wn, lr, hi);
+            else store<MT, NP, OUT>(acc, p, m0, n0, wm, wn, lr, hi);
             kb = 0;
             tile += grid;
         }
@@ -670,14 +671,20 @@ __global__ void __launch_bounds__(256) k_sum_slices(Fp8Args p, int slices) {
     if (at >= size) return;
     OUT* out = static_cast<OUT*>(p.out);
     const OUT* bias = static_cast<const OUT*>(p.bias);
-    if (p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & (4 * sizeof(OUT) - 1)) == 0) {
+    if (at + 4 <= size && p.n >= 4) {
+        typedef f32x4_t Any __attribute__((aligned(4)));
         f32x4_t v = *reinterpret_cast<const f32x4_t*>(p.part + at);
-        for (int s = 1; s < slices; ++s) v += *reinterpret_cast<const f32x4_t*>(p.part + s * size + at);
+        for (int s = 1; s < slices; ++s) v += *reinterpret_cast<const Any*>(p.part + s * size + at);
         const int64_t col = at % p.n;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = act_out<OUT>(bias ? v[e] + ld_out(bias + col + e) : v[e], p.act);
-        if constexpr (sizeof(OUT) == 4) *reinterpret_cast<f32x4_t*>(out + at) = v;
-        else *reinterpret_cast<uint2*>(out + at) = make_uint2(f2bf2(v[0], v[1]), f2bf2(v[2], v[3]));
+        for (int e = 0; e < 4; ++e)
+            v[e] = act_out<OUT>(bias ? v[e] + ld_out(bias + (col + e < p.n ? col + e : col + e - p.n)) : v[e], p.act);
+        if constexpr (sizeof(OUT) == 4) {
+            store16<false>(v, out + at);
+        } else {
+            typedef uint32_t Pair __attribute__((ext_vector_type(2)));
+            store16<false>(Pair{f2bf2(v[0], v[1]), f2bf2(v[2], v[3])}, out + at);
+        }
         return;
     }
     for (int64_t i = at; i < min(at + 4, size); ++i) {

@@ -24,25 +24,29 @@ constexpr float kE4m3Max = 448.0f;
 constexpr uint32_t kAmaxFloorBits = 0x0f800000u;   // 2^-96
 constexpr int kThreads = 256;
 
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
 __device__ __forceinline__ float value(float v) { return v; }
 __device__ __forceinline__ float value(bf16_t v) { return bf2f(v); }
 
-// Eight values at column `col` of a row (its address `p` is that of `col`), zero from column `cols` on.
-template <typename T, bool VEC>
+// Eight values at column `col` of a row (its address `p` is that of `col`), zero from column `cols` on. Memory takes 16 bytes
+// at the alignment of a value, so rows of any stride load alike (8192 x 4607 bf16: 27 us, value by value 52).
+template <typename T>
 __device__ __forceinline__ void load8(const T* p, int64_t col, int64_t cols, float (&v)[8]) {
-    if (VEC && col + 8 <= cols) {
+    if (col + 8 <= cols) {
         if constexpr (sizeof(T) == 2) {
-            const uint4 r = *reinterpret_cast<const uint4*>(p);
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+            typedef u32x4_t Any __attribute__((aligned(2)));
+            const u32x4_t w = *reinterpret_cast<const Any*>(p);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 v[2 * i] = __uint_as_float(w[i] << 16);
                 v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
             }
         } else {
+            typedef f32x4_t Any __attribute__((aligned(4)));
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const f32x4_t r = *reinterpret_cast<const f32x4_t*>(p + 4 * i);
+                const f32x4_t r = *reinterpret_cast<const Any*>(p + 4 * i);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[4 * i + e] = r[e];
             }
@@ -88,7 +92,7 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], float factor, int64
 // Workgroup: 16 rows x 512 columns. A wave takes four rows, its 64 lanes a row's 512 columns (eight
 // values each, 16 lanes a block), all four rows' loads before the first maximum. The scales are laid
 // out [block of columns, row] and leave through LDS, 16 consecutive rows a block.
-template <typename T, bool VEC>
+template <typename T>
 __global__ void __launch_bounds__(kThreads) k_quantize_rows(const T* __restrict__ x, int64_t ld, uint8_t* __restrict__ q,
                                                             int64_t ld_q, float* __restrict__ scales, int64_t rows,
                                                             int64_t cols, int64_t col_blocks) {
@@ -101,7 +105,7 @@ __global__ void __launch_bounds__(kThreads) k_quantize_rows(const T* __restrict_
     for (int r = 0; r < 4; ++r) {
         const int64_t row = r0 + wave * 4 + r;
         const int64_t lim = row < rows ? cols : 0;
-        load8<T, VEC>(x + min(row, rows - 1) * ld + col, col, lim, v[r]);
+        load8<T>(x + min(row, rows - 1) * ld + col, col, lim, v[r]);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -120,7 +124,7 @@ __global__ void __launch_bounds__(kThreads) k_quantize_rows(const T* __restrict_
 }
 
 // Workgroup: one 128 x 128 block, 64 values a thread in registers.
-template <typename T, bool VEC>
+template <typename T>
 __global__ void __launch_bounds__(kThreads) k_quantize_blocks(const T* __restrict__ x, int64_t ld, uint8_t* __restrict__ q,
                                                               int64_t ld_q, float* __restrict__ scales, int64_t rows,
                                                               int64_t cols, int64_t col_blocks) {
@@ -133,7 +137,7 @@ __global__ void __launch_bounds__(kThreads) k_quantize_blocks(const T* __restric
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
         const int64_t row = row0 + p * 16;
-        load8<T, VEC>(x + min(row, rows - 1) * ld + col, col, row < rows ? cols : 0, v[p]);
+        load8<T>(x + min(row, rows - 1) * ld + col, col, row < rows ? cols : 0, v[p]);
     }
 #pragma unroll
     for (int p = 0; p < 8; ++p) m = max(m, amax8(v[p]));
@@ -154,13 +158,11 @@ __global__ void __launch_bounds__(kThreads) k_quantize_blocks(const T* __restric
 
 template <typename T>
 void quantize(const T* x, int64_t ld, uint8_t* q, float* scales, int64_t rows, int64_t cols, bool blocks, hipStream_t s) {
-    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * static_cast<int64_t>(sizeof(T)) % 16 == 0;
     const int64_t ld_q = fp8_row_bytes(cols);
     const int64_t col_blocks = blocks ? (cols + 127) / 128 : (cols + 511) / 512;
     const int64_t grid = col_blocks * (blocks ? (rows + 127) / 128 : (rows + 15) / 16);
     require(grid < (int64_t{1} << 31), "quantize_fp8: the matrix is too large");
-    auto* kernel = blocks ? (vec ? &k_quantize_blocks<T, true> : &k_quantize_blocks<T, false>)
-                          : (vec ? &k_quantize_rows<T, true> : &k_quantize_rows<T, false>);
+    auto* kernel = blocks ? &k_quantize_blocks<T> : &k_quantize_rows<T>;
     kernel<<<static_cast<unsigned>(grid), kThreads, 0, s>>>(x, ld, q, ld_q, scales, rows, cols, col_blocks);
     launch_check("quantize_fp8");
 }
