@@ -264,6 +264,18 @@ def test_gemm_outliers_and_no_workspace(hip, m, n, k, dtype):
     check_gemm(m, n, k, dtype=dtype, workspace=False)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("m,n,k", [(3, 300, 300), (300, 257, 400), (500, 1028, 640), (300, 130, 8192)])
+def test_gemm_bias_of_any_alignment(hip, m, n, k, dtype):
+    import torch
+    a, sa, b, sb = operands(m, n, k, 5)
+    wide = normal((n + 9,), 3, getattr(torch, dtype))
+    for shift in (1, 3, 8):
+        bias = wide[shift:shift + n]
+        want, tol = gemm_plain(a, sa, b, sb, bias, k, 1, dtype)
+        assert ((run_gemm(a, sa, b, sb, bias, k, 1, dtype).double() - want).abs() <= tol).all()
+
+
 def test_gemm_of_an_empty_sum_is_the_epilogue_of_the_bias(hip):
     import torch
     one = torch.zeros(64, dtype=torch.uint8, device="cuda")
