@@ -594,17 +594,16 @@ int device_cus() {
 }
 
 // How a call runs: k_window_many, or k_window_few on tiles of 16 `few` rows with the keys in `splits`. The estimates, in
-// us, were fitted to 20 shapes on one MI355X (head_dim 64 to 128, 1 to 2000 rows of 300 to 16000 keys), each on every
-// kernel and split that fits it; what they choose is within 6% of the fastest there but for 1.14 once (4 x 2 key heads x
-// 1200 rows, window 64: 13.0 against 11.4). Beside 3.5 a workgroup,
+// us, were checked on 35 shapes on one MI355X (head_dim 32 to 128, 1 to 2048 rows of 77 to 16000 keys), each on every
+// kernel and split that fits it: what they choose is within 5% of the fastest. Beside 3.5 a workgroup,
 //  - many: a block of 64 keys costs 0.62 + 0.006 head_dim alone on a CU, 0.5 + 0.014 beside another workgroup;
-//  - few: a piece of 32 keys for each of the four waves costs 0.35 + 0.005 head_dim on 16 rows, 0.3 + 0.009 on 32,
-//    0.35 + 0.0165 on 64, one workgroup a CU (two up to head_dim 64), and no less in all than reading the keys at
+//  - few: a piece of 32 keys for each of the four waves costs 0.35 + 0.005 head_dim on 16 rows and 0.3 + 0.009 on 32, one
+//    workgroup a CU (two up to head_dim 64), and no less in all than reading the keys at
 //    5.2 TB/s (a quarter more on fewer workgroups than CUs);
 //  - a join costs 3 + 0.25 a split and its partial results at 3 TB/s.
 // 16 sequences of a token each, 32 / 8 heads of 128, 4096 keys: two splits 57 us, none 65, k_window_many 90. Four times
-// 64 tokens of the same: 32-row tiles 52, 16-row 82, 64-row 80, k_window_many 97. 2 x 64 heads of 300 tokens, head_dim 64:
-// k_window_many 15.6, 32-row tiles 24.
+// 64 tokens of the same: 32-row tiles 52, 16-row 82, k_window_many 88. 2 x 64 heads of 300 tokens, head_dim 64:
+// k_window_many 15.5, 32-row tiles 24. (64-row tiles were never ahead of these, 55 and 33 there.)
 struct Plan {
     int few;      // 0: k_window_many
     int splits;
@@ -625,10 +624,10 @@ Plan plan(const WindowShape& sh, bool may_split) {
         const double blocks = static_cast<double>(up(keys(kManyRows), kKeys));
         least = groups <= cus ? 3.5 + blocks * (0.62 + 0.006 * D) : up(groups, 2 * cus) * (3.5 + blocks * (0.5 + 0.014 * D));
     }
-    for (int few : {1, 2, 4}) {
-        if (few > 1 && rows <= 8 * few) continue;
+    for (int few : {1, 2}) {
+        if (few > 1 && rows <= 16) continue;
         const int64_t pieces = up(keys(16 * few), kPiece);
-        const double step = few == 1 ? 0.35 + 0.005 * D : few == 2 ? 0.3 + 0.009 * D : 0.35 + 0.0165 * D;
+        const double step = few == 1 ? 0.35 + 0.005 * D : 0.3 + 0.009 * D;
         for (int s = 1; s == 1 || (may_split && s <= 32 && 4 * s <= pieces); s *= 2) {
             const int64_t groups = heads * up(rows, 16 * few) * s, at_once = cus * (sh.head_dim <= 64 ? 2 : 1);
             const double bytes = static_cast<double>(heads) * keys(rows) * D * 4;
@@ -648,8 +647,7 @@ void launch(const WindowArgs& a, const Plan& how, int64_t grid, hipStream_t s) {
     const unsigned n = static_cast<unsigned>(grid);
     if (how.few == 0) k_window_many<DT><<<n, kThreads, 0, s>>>(a);
     else if (how.few == 1) k_window_few<DT, 1><<<n, kThreads, 0, s>>>(a);
-    else if (how.few == 2) k_window_few<DT, 2><<<n, kThreads, 0, s>>>(a);
-    else k_window_few<DT, 4><<<n, kThreads, 0, s>>>(a);
+    else k_window_few<DT, 2><<<n, kThreads, 0, s>>>(a);
 }
 
 }  // namespace
