@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kWaves * 64) k_gemm_fp8_rows(Fp8Args a) {
 // Measured: 8192 x 8192 x 8192 1.95 us a 256 x 256 x 128 block, two waves a SIMD at 65% of the matrix instruction's own
 // rate (what is left is LDS reads and issue; loads are not waited for); 8192 x 8192 x 1152 94 us (1650 TFLOP/s), 8192 x
 // 4608 x 1152 57 to 62 us, where the nine blocks of K end in stores that all workgroups issue together; 600 x 4096 x 10240
-// in three slices 43 us. fp32 outputs, through bf16 products: 8192 x 8192 x 2048 268 us (1026 TFLOP/s), of which
+// in three slices 41 to 43 us. fp32 outputs, through bf16 products: 8192 x 8192 x 2048 268 us (1026 TFLOP/s), of which
 // widening the codes is 12%.
 namespace tile {
 
@@ -724,10 +724,12 @@ int device_cus() {
 
 // How a product runs: `mt` 16-row tiles of the rows kernel, or 64 mt x 64 np tiles with K in `slices`. Estimated
 // times in ns. Fitted to one MI355X, 8192 x 8192 x 4096 on each tile: a block of K costs a workgroup 1.56 an
-// operand row and 0.0176 an output (twice that through bf16 operands), a tile's end 0.085 a bf16 output and
-// twice that an fp32 one: 256 x 256 tiles 1.95 us a block, 256 x 192 1.56 (measured 1.45), 256 x 128 1.18,
-// 128 x 192 0.93, 128 x 128 0.69. Slices add a launch and their fp32 sums, written and read. The rows kernel
-// takes 100, 140 or 280 for a block of K of 16 columns and 16, 32 or 64 rows.
+// operand row and 0.0176 an output (twice that through bf16 operands), a tile's end 0.072 a bf16 output and
+// 0.16 an fp32 one: 256 x 256 tiles 1.95 us a block, 256 x 192 1.56 (measured 1.45), 256 x 128 1.18,
+// 128 x 192 0.93, 128 x 128 0.69. Slices add a launch, 2400, and their fp32 sums, written and read. The rows kernel
+// takes 140 or 250 for a block of K of 16 columns and 16 or 32, or 64 rows. What that chooses is within 7% of the fastest
+// tile and number of slices on 63 of 64 products of 24 to 8192 rows, both output types (the other 14%: 128 x 4096 x 4096,
+// eight slices 20.0 us, three 17.5).
 struct Plan {
     bool tiles;
     int mt, np, slices;
@@ -738,7 +740,7 @@ Plan plan(int64_t m, int64_t n, int64_t k, bool f32, bool may_split) {
     Plan best{false, rows_mt, 0, 1};
     if (m <= 16 || blocks == 0 || k >= (int64_t{1} << 22)) return best;   // 32-bit offsets inside a tile
     const double groups = static_cast<double>((n + 15) / 16) * ((m + 16 * rows_mt - 1) / (16 * rows_mt));
-    double least = std::max(1.0, groups / cus) * blocks * (rows_mt == 4 ? 280 : 140);
+    double least = std::max(1.0, groups / cus) * blocks * (rows_mt == 4 ? 250 : 140);
     static constexpr int kTiles[][2] = {{4, 4}, {4, 3}, {4, 2}, {2, 4}, {2, 3}, {2, 2}};
     for (const auto& tile : kTiles) {
         const int64_t bm = 64 * tile[0], bn = 64 * tile[1], tiles = ((m + bm - 1) / bm) * ((n + bn - 1) / bn);
@@ -747,8 +749,8 @@ Plan plan(int64_t m, int64_t n, int64_t k, bool f32, bool may_split) {
             const int64_t at_once = std::max<int64_t>(1, cus / s);
             const double rounds = static_cast<double>((tiles + at_once - 1) / at_once);
             double cost = rounds * ((blocks + s - 1) / s * (1.56 * (bm + bn) + (f32 ? 0.0352 : 0.0176) * bm * bn) +
-                                    (f32 || s > 1 ? 0.17 : 0.085) * bm * bn);
-            if (s > 1) cost += 3000 + (s * 4 + (f32 ? 4 : 2)) * static_cast<double>(m) * n / 4500;
+                                    (f32 || s > 1 ? 0.16 : 0.072) * bm * bn);
+            if (s > 1) cost += 2400 + (s * 4 + (f32 ? 4 : 2)) * static_cast<double>(m) * n / 5300;
             if (cost < least) {
                 least = cost;
                 best = Plan{true, tile[0], tile[1], s};
