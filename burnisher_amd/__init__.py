@@ -97,6 +97,15 @@ class ProbeResult(ctypes.Structure):
         return {f: (round(getattr(self, f), 2) if f != "cus" else self.cus) for f, _ in self._fields_}
 
 
+class GemmFp8Plan(ctypes.Structure):
+    _fields_ = [("in_lds", ctypes.c_int), ("tile_rows", ctypes.c_int), ("tile_cols", ctypes.c_int),
+                ("slices", ctypes.c_int), ("tiles", ctypes.c_int64), ("workgroups", ctypes.c_int64)]
+
+
+class AttentionWindowPlan(ctypes.Structure):
+    _fields_ = [("tile_rows", ctypes.c_int), ("splits", ctypes.c_int), ("workgroups", ctypes.c_int64)]
+
+
 class SchedCoefficients(ctypes.Structure):
     _fields_ = [("order", ctypes.c_int)] + [
         (f, ctypes.c_double) for f in ("sigma_s0", "sigma_t", "sigma_vp_s0", "sigma_vp_t",
@@ -138,9 +147,11 @@ SIGNATURES = {
     "bh_quantize_fp8": ([_V, _I64, _V, _V, _I64, _I64, _I, _I, _V], _I),
     "bh_gemm_fp8": ([_V, _V, _V, _V, _V, _V, _I64, _I64, _I64, _I, _I, _V, _I64, _V], _I),
     "bh_gemm_fp8_workspace_bytes": ([_I64, _I64, _I64], _I64),
+    "bh_gemm_fp8_describe": ([_I64, _I64, _I64, _I, _I, _I, ctypes.POINTER(GemmFp8Plan)], _I),
     "bh_attention_window": ([_V, _I64, _V, _V, _I64, _V, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _I64,
                              _I64, _I64, _V, _V, _I, _V, _I64, _V], _I),
     "bh_attention_window_workspace_bytes": ([_I64] * 9, _I64),
+    "bh_attention_window_describe": ([_I64] * 9 + [_I, _I, ctypes.POINTER(AttentionWindowPlan)], _I),
     "bh_scale": ([_V, _V, _I64, _F, _I, _V], _I),
     "bh_timestep_embedding": ([_D, _I, _I64, _V, _I, _V], _I),
     "bh_probe_device": ([_V, _V, _I64, ctypes.POINTER(ProbeResult)], _I),

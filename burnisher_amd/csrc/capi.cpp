@@ -416,6 +416,21 @@ int bh_gemm_fp8(const void* a, const float* a_scales, const void* b, const float
     });
 }
 
+int bh_gemm_fp8_describe(int64_t m, int64_t n, int64_t k, int dtype, int with_workspace, int cus,
+                         bh_gemm_fp8_plan* out) {
+    return guarded([&] {
+        const char* op = "gemm_fp8_describe";
+        require_nonneg(m, op, "m");
+        require_nonneg(n, op, "n");
+        require_nonneg(k, op, "k");
+        require(m < kSizeLimit && n < kSizeLimit && k < kSizeLimit, "gemm_fp8_describe: m, n and k must be below 2^30");
+        require(cus >= 0, "gemm_fp8_describe: cus is negative");
+        require(out != nullptr, "gemm_fp8_describe: out is null");
+        const bool f32 = is_f32(dtype);
+        *out = m * n == 0 ? bh_gemm_fp8_plan{} : gemm_fp8_plan(m, n, k, f32, with_workspace != 0, cus);
+    });
+}
+
 namespace {
 WindowShape window_shape(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
                          int64_t head_dim, int64_t left, int64_t right, int64_t sinks) {
@@ -448,6 +463,18 @@ int64_t bh_attention_window_workspace_bytes(int64_t batch, int64_t heads, int64_
         bytes = batch * heads * q_len == 0 ? 0 : 4 * attention_window_workspace_floats(sh);
     });
     return bytes;
+}
+
+int bh_attention_window_describe(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                                 int64_t head_dim, int64_t window_left, int64_t window_right, int64_t sinks,
+                                 int with_workspace, int cus, bh_attention_window_plan* out) {
+    return guarded([&] {
+        const WindowShape sh = window_shape(batch, heads, kv_heads, q_len, kv_len, head_dim, window_left, window_right,
+                                            sinks);
+        require(cus >= 0, "attention_window_describe: cus is negative");
+        require(out != nullptr, "attention_window_describe: out is null");
+        *out = batch * heads * q_len == 0 ? bh_attention_window_plan{} : attention_window_plan(sh, with_workspace != 0, cus);
+    });
 }
 
 int bh_attention_window(const void* q, int64_t ld_q, const void* k, const void* v, int64_t ld_kv,

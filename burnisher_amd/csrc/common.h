@@ -559,6 +559,8 @@ void launch_quantize_fp8(const void* x, int64_t ld, uint8_t* q, float* scales, i
                          bool f32, hipStream_t s);
 // Floats of workspace that a product of these sizes uses when it has one (0: none).
 int64_t gemm_fp8_workspace_floats(int64_t m, int64_t n, int64_t k, bool f32);
+// How launch_gemm_fp8 runs such a product (`may_split`: with a workspace) on a device of `cus` CUs (0: the current one).
+bh_gemm_fp8_plan gemm_fp8_plan(int64_t m, int64_t n, int64_t k, bool f32, bool may_split, int cus);
 // bias and out are fp32 with f32, else bf16. `ws`: those floats, or null to run without.
 void launch_gemm_fp8(const uint8_t* a, const float* sa, const uint8_t* b, const float* sb, const void* bias, void* out,
                      int64_t m, int64_t n, int64_t k, int act, bool f32, float* ws, hipStream_t s);
@@ -570,6 +572,8 @@ struct WindowShape {
 };
 // Floats of workspace that a call of this shape uses when it has one (0: none).
 int64_t attention_window_workspace_floats(const WindowShape& sh);
+// How launch_attention_window runs such a call, as gemm_fp8_plan.
+bh_attention_window_plan attention_window_plan(const WindowShape& sh, bool may_split, int cus);
 void launch_attention_window(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16_t* out, const WindowShape& sh,
                              const int32_t* kv_lens, const int32_t* q_starts, float* ws, hipStream_t s);
 

@@ -696,10 +696,10 @@ __global__ void __launch_bounds__(256) k_sum_slices(Fp8Args p, int slices) {
 }
 
 template <int MT, int NP, bool EXACT, typename OUT>
-void launch(const Fp8Args& p, int slices, int cus, hipStream_t s) {
+void launch(const Fp8Args& p, int slices, int64_t workgroups, hipStream_t s) {
     const int tiles_m = static_cast<int>((p.m + 64 * MT - 1) / (64 * MT)), tiles_n = static_cast<int>((p.n + 64 * NP - 1) / (64 * NP));
-    const int grid = std::min(tiles_m * tiles_n, std::max(cus / slices & ~7, 1));
-    k_gemm_fp8_tile<MT, NP, EXACT, OUT><<<dim3(grid, slices), kThreads, 0, s>>>(p, tiles_m, tiles_n, std::max(1, 16 / MT));
+    k_gemm_fp8_tile<MT, NP, EXACT, OUT>
+        <<<dim3(static_cast<unsigned>(workgroups), slices), kThreads, 0, s>>>(p, tiles_m, tiles_n, std::max(1, 16 / MT));
     if (slices == 1) return;
     launch_check("gemm_fp8");
     const int64_t blocks = (p.m * p.n + 1023) / 1024;
@@ -722,6 +722,14 @@ int device_cus() {
     return n;
 }
 
+// Workgroups that walk a slice's tiles, one a CU at once. A multiple of eight keeps the tiles that a workgroup goes on
+// to on its XCD, but not where that many would take a round more.
+int64_t workgroups(int64_t tiles, int slices, int64_t cus) {
+    const int64_t most = std::max<int64_t>(1, cus / slices), even = most & ~int64_t{7};
+    auto rounds = [&](int64_t n) { return (tiles + n - 1) / n; };
+    return std::min(tiles, even > 0 && rounds(even) == rounds(most) ? even : most);
+}
+
 // How a product runs: `mt` 16-row tiles of the rows kernel, or 64 mt x 64 np tiles with K in `slices`. Estimated
 // times in ns. Fitted to one MI355X, 8192 x 8192 x 4096 on each tile: a block of K costs a workgroup 1.56 an
 // operand row and 0.0176 an output (twice that through bf16 operands), a tile's end 0.072 a bf16 output and
@@ -733,27 +741,28 @@ int device_cus() {
 struct Plan {
     bool tiles;
     int mt, np, slices;
+    int64_t groups;   // workgroups, of each slice
 };
-Plan plan(int64_t m, int64_t n, int64_t k, bool f32, bool may_split) {
-    const int64_t blocks = (k + 127) / 128, cus = device_cus();
+Plan plan(int64_t m, int64_t n, int64_t k, bool f32, bool may_split, int64_t cus) {
+    const int64_t blocks = (k + 127) / 128;
     const int rows_mt = m > 32 ? 4 : m > 16 ? 2 : 1;
-    Plan best{false, rows_mt, 0, 1};
+    const int64_t groups = (n + 15) / 16 * ((m + 16 * rows_mt - 1) / (16 * rows_mt));
+    Plan best{false, rows_mt, 0, 1, groups};
     if (m <= 16 || blocks == 0 || k >= (int64_t{1} << 22)) return best;   // 32-bit offsets inside a tile
-    const double groups = static_cast<double>((n + 15) / 16) * ((m + 16 * rows_mt - 1) / (16 * rows_mt));
-    double least = std::max(1.0, groups / cus) * blocks * (rows_mt == 4 ? 250 : 140);
+    double least = std::max(1.0, static_cast<double>(groups) / cus) * blocks * (rows_mt == 4 ? 250 : 140);
     static constexpr int kTiles[][2] = {{4, 4}, {4, 3}, {4, 2}, {2, 4}, {2, 3}, {2, 2}};
     for (const auto& tile : kTiles) {
         const int64_t bm = 64 * tile[0], bn = 64 * tile[1], tiles = ((m + bm - 1) / bm) * ((n + bn - 1) / bn);
         if (tiles >= (int64_t{1} << 31) || (f32 && tile[0] + tile[1] > 7)) continue;   // 256 x 256 in fp32 spills
         for (int s = 1; s <= (may_split ? 8 : 1) && s <= blocks; ++s) {
-            const int64_t at_once = std::max<int64_t>(1, cus / s);
+            const int64_t at_once = workgroups(tiles, s, cus);
             const double rounds = static_cast<double>((tiles + at_once - 1) / at_once);
             double cost = rounds * ((blocks + s - 1) / s * (1.56 * (bm + bn) + (f32 ? 0.0352 : 0.0176) * bm * bn) +
                                     (f32 || s > 1 ? 0.16 : 0.072) * bm * bn);
             if (s > 1) cost += 2400 + (s * 4 + (f32 ? 4 : 2)) * static_cast<double>(m) * n / 5300;
             if (cost < least) {
                 least = cost;
-                best = Plan{true, tile[0], tile[1], s};
+                best = Plan{true, tile[0], tile[1], s, at_once};
             }
         }
     }
@@ -763,22 +772,28 @@ Plan plan(int64_t m, int64_t n, int64_t k, bool f32, bool may_split) {
 }  // namespace
 
 int64_t gemm_fp8_workspace_floats(int64_t m, int64_t n, int64_t k, bool f32) {
-    const Plan p = plan(m, n, k, f32, true);
+    const Plan p = plan(m, n, k, f32, true, device_cus());
     return p.slices > 1 ? p.slices * m * n : 0;
+}
+
+bh_gemm_fp8_plan gemm_fp8_plan(int64_t m, int64_t n, int64_t k, bool f32, bool may_split, int cus) {
+    const Plan p = plan(m, n, k, f32, may_split, cus > 0 ? cus : device_cus());
+    const int rows = p.tiles ? 64 * p.mt : 16 * p.mt, cols = p.tiles ? 64 * p.np : 16;
+    return bh_gemm_fp8_plan{p.tiles ? 1 : 0, rows, cols, p.slices, (m + rows - 1) / rows * ((n + cols - 1) / cols), p.groups};
 }
 
 void launch_gemm_fp8(const uint8_t* a, const float* sa, const uint8_t* b, const float* sb, const void* bias, void* out,
                      int64_t m, int64_t n, int64_t k, int act, bool f32, float* ws, hipStream_t s) {
     Fp8Args p{a, sa, b, sb, bias, out, m, n, fp8_row_bytes(k), static_cast<int>((k + 127) / 128), act, ws};
     ProfileScope ps(K_GEMM, s, 2.0 * m * n * k);
-    const Plan how = plan(m, n, k, f32, ws != nullptr);
+    const Plan how = plan(m, n, k, f32, ws != nullptr, device_cus());
     if (how.tiles) {
         auto go = [&](auto mt, auto np) {
             constexpr int MT = decltype(mt)::value, NP = decltype(np)::value;
             if constexpr (MT + NP <= 7) {
-                if (f32) return tile::launch<MT, NP, true, float>(p, how.slices, device_cus(), s);
+                if (f32) return tile::launch<MT, NP, true, float>(p, how.slices, how.groups, s);
             }
-            tile::launch<MT, NP, false, bf16_t>(p, how.slices, device_cus(), s);
+            tile::launch<MT, NP, false, bf16_t>(p, how.slices, how.groups, s);
         };
         constexpr std::integral_constant<int, 2> two;
         constexpr std::integral_constant<int, 3> three;
@@ -789,7 +804,7 @@ void launch_gemm_fp8(const uint8_t* a, const float* sa, const uint8_t* b, const 
         return;
     }
     const int mt = how.mt;
-    const int64_t grid = (n + 15) / 16 * ((m + 16 * mt - 1) / (16 * mt));
+    const int64_t grid = how.groups;
     require(grid < (int64_t{1} << 31), "gemm_fp8: the output is too large");
     auto launch = [&](void (*kernel)(Fp8Args)) { kernel<<<static_cast<unsigned>(grid), kWaves * 64, 0, s>>>(p); };
     if (mt == 1) launch(f32 ? &k_gemm_fp8_rows<1, true, float> : &k_gemm_fp8_rows<1, false, bf16_t>);

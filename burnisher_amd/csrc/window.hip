@@ -608,8 +608,8 @@ struct Plan {
     int few;      // 0: k_window_many
     int splits;
 };
-Plan plan(const WindowShape& sh, bool may_split) {
-    const int64_t cus = device_cus(), group = sh.heads / sh.kv_heads, rows = group * sh.q_len, heads = sh.batch * sh.kv_heads;
+Plan plan(const WindowShape& sh, bool may_split, int64_t cus) {
+    const int64_t group = sh.heads / sh.kv_heads, rows = group * sh.q_len, heads = sh.batch * sh.kv_heads;
     const double D = static_cast<double>(sh.head_dim);
     auto keys = [&](int64_t n) {   // that n rows see at most
         if (sh.left < 0 || sh.right < 0) return sh.kv_len;
@@ -642,6 +642,8 @@ Plan plan(const WindowShape& sh, bool may_split) {
     return best;
 }
 
+int tile_rows(const Plan& how) { return how.few == 0 ? kManyRows : 16 * how.few; }
+
 template <int DT>
 void launch(const WindowArgs& a, const Plan& how, int64_t grid, hipStream_t s) {
     const unsigned n = static_cast<unsigned>(grid);
@@ -653,9 +655,15 @@ void launch(const WindowArgs& a, const Plan& how, int64_t grid, hipStream_t s) {
 }  // namespace
 
 int64_t attention_window_workspace_floats(const WindowShape& sh) {
-    const Plan how = plan(sh, true);
+    const Plan how = plan(sh, true, device_cus());
     if (how.splits == 1) return 0;
     return how.splits * sh.batch * sh.heads * sh.q_len * (sh.head_dim + 2);
+}
+
+bh_attention_window_plan attention_window_plan(const WindowShape& sh, bool may_split, int cus) {
+    const Plan how = plan(sh, may_split, cus > 0 ? cus : device_cus());
+    const int64_t rows = sh.heads / sh.kv_heads * sh.q_len, per = tile_rows(how), tiles = (rows + per - 1) / per;
+    return bh_attention_window_plan{static_cast<int>(per), how.splits, tiles * sh.batch * sh.kv_heads * how.splits};
 }
 
 void launch_attention_window(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16_t* out, const WindowShape& sh,
@@ -670,8 +678,8 @@ void launch_attention_window(const bf16_t* q, const bf16_t* k, const bf16_t* v, 
     a.Sq = static_cast<int>(sh.q_len); a.Skv = static_cast<int>(sh.kv_len); a.D = static_cast<int>(sh.head_dim);
     a.left = sh.left; a.right = sh.right; a.sinks = sh.sinks;
     a.c = sh.scale * kLog2e;
-    const Plan how = plan(sh, ws != nullptr);
-    const int64_t rows = static_cast<int64_t>(a.group) * a.Sq, per = how.few == 0 ? kManyRows : 16 * how.few, tiles = (rows + per - 1) / per;
+    const Plan how = plan(sh, ws != nullptr, device_cus());
+    const int64_t rows = static_cast<int64_t>(a.group) * a.Sq, per = tile_rows(how), tiles = (rows + per - 1) / per;
     a.tiles = static_cast<int>(tiles);
     a.splits = how.splits;
     const int64_t grid = tiles * sh.batch * sh.kv_heads * how.splits;

@@ -217,6 +217,19 @@ int bh_gemm_fp8(const void* a, const float* a_scales, const void* b, const float
                 void* workspace, int64_t workspace_bytes, void* stream);
 int64_t bh_gemm_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k);
 
+/* How bh_gemm_fp8 runs a product of these sizes, with a workspace or without, on a device of `cus`
+ * compute units (0: the current device): what a log or a test wants to know. An empty product has all
+ * zeros. Which form a size takes may change from one build of the library to the next. */
+typedef struct bh_gemm_fp8_plan {
+    int in_lds;                 /* 1: tiles out of LDS; 0: operands straight from memory (few rows) */
+    int tile_rows, tile_cols;   /* of the output, a workgroup's at a time */
+    int slices;                 /* of K; above 1 the workspace takes their sums */
+    int64_t tiles;
+    int64_t workgroups;         /* of a slice; each walks tiles / workgroups of them, rounded up */
+} bh_gemm_fp8_plan;
+int bh_gemm_fp8_describe(int64_t m, int64_t n, int64_t k, int dtype, int with_workspace, int cus,
+                         bh_gemm_fp8_plan* out);
+
 /* Attention through a sliding window, with first keys that stay visible and grouped heads; bf16.
  * Query head h reads key head h / (heads / kv_heads). Query i of batch row b stands at position
  * p = q_starts[b] + i and sees key j when
@@ -242,6 +255,16 @@ int bh_attention_window(const void* q, int64_t ld_q, const void* k, const void* 
 int64_t bh_attention_window_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
                                             int64_t q_len, int64_t kv_len, int64_t head_dim,
                                             int64_t window_left, int64_t window_right, int64_t sinks);
+
+/* The same of a bh_attention_window call, as bh_gemm_fp8_describe. */
+typedef struct bh_attention_window_plan {
+    int tile_rows;        /* of (token, head of a group): 128 share their keys in LDS, 16 or 32 read them wave by wave */
+    int splits;           /* workgroups that share a tile's keys; above 1 the workspace takes their results */
+    int64_t workgroups;
+} bh_attention_window_plan;
+int bh_attention_window_describe(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                                 int64_t head_dim, int64_t window_left, int64_t window_right, int64_t sinks,
+                                 int with_workspace, int cus, bh_attention_window_plan* out);
 
 /* ---- device probe ---------------------------------------------------------------------------- */
 
