@@ -98,7 +98,8 @@ __global__ void __launch_bounds__(kThreads) k_quantize_rows(const T* __restrict_
                                                             int64_t cols, int64_t col_blocks) {
     __shared__ float s[4][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
-    const int64_t cb = blockIdx.x % col_blocks, r0 = blockIdx.x / col_blocks * 16;
+    const int64_t id = group_index(), cb = id % col_blocks, r0 = id / col_blocks * 16;
+    if (r0 >= rows) return;
     const int64_t col = cb * 512 + lane * 8;
     float v[4][8];
 #pragma unroll
@@ -130,7 +131,8 @@ __global__ void __launch_bounds__(kThreads) k_quantize_blocks(const T* __restric
                                                               int64_t cols, int64_t col_blocks) {
     __shared__ uint32_t s[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t cb = blockIdx.x % col_blocks, rb = blockIdx.x / col_blocks;
+    const int64_t id = group_index(), cb = id % col_blocks, rb = id / col_blocks;
+    if (rb * 128 >= rows) return;
     const int64_t col = cb * 128 + (lane & 15) * 8, row0 = rb * 128 + wave * 4 + (lane >> 4);
     float v[8][8];
     uint32_t m = 0;
@@ -163,7 +165,7 @@ void quantize(const T* x, int64_t ld, uint8_t* q, float* scales, int64_t rows, i
     const int64_t grid = col_blocks * (blocks ? (rows + 127) / 128 : (rows + 15) / 16);
     require(grid < (int64_t{1} << 31), "quantize_fp8: the matrix is too large");
     auto* kernel = blocks ? &k_quantize_blocks<T> : &k_quantize_rows<T>;
-    kernel<<<static_cast<unsigned>(grid), kThreads, 0, s>>>(x, ld, q, ld_q, scales, rows, cols, col_blocks);
+    kernel<<<grid_of(grid, kThreads), kThreads, 0, s>>>(x, ld, q, ld_q, scales, rows, cols, col_blocks);
     launch_check("quantize_fp8");
 }
 

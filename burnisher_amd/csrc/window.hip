@@ -284,7 +284,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_window_many(WindowArgs a) {
     __shared__ __attribute__((aligned(1024))) char kmem[2 * kKBytes], vmem[2 * kVBytes];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int T = a.tiles * a.B * a.KH;
-    int id = blockIdx.x;
+    int id = static_cast<int>(group_index());
+    if (id >= T) return;
     if ((T & 7) == 0) id = (id & 7) * (T >> 3) + (id >> 3);   // neighbouring tiles, which share keys, on one XCD
     const int tile = id % a.tiles, bk = id / a.tiles, kh = bk % a.KH, b = bk / a.KH;
     const int rows = a.group * a.Sq, row0 = tile * kManyRows, row1 = min(row0 + kManyRows, rows) - 1;
@@ -440,8 +441,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_window_few(WindowArgs a) {
     static_assert(kItems <= 60, "vmcnt");
     __shared__ __attribute__((aligned(1024))) char smem[4 * 2 * kStage];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int T = gridDim.x;
-    int id = blockIdx.x;
+    const int T = a.tiles * a.splits * a.B * a.KH;
+    int id = static_cast<int>(group_index());
+    if (id >= T) return;
     if ((T & 7) == 0) id = (id & 7) * (T >> 3) + (id >> 3);   // tiles that read the same keys on one XCD
     const int tile = id % a.tiles, split = id / a.tiles % a.splits, bk = id / a.tiles / a.splits, kh = bk % a.KH, b = bk / a.KH;
     const int rows = a.group * a.Sq, row0 = tile * (16 * QT), row1 = min(row0 + 16 * QT, rows) - 1;
@@ -560,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_window_few(WindowArgs a) {
 __global__ void __launch_bounds__(kThreads) k_window_join(WindowArgs a) {
     const int rows = a.group * a.Sq;
     const int64_t all = static_cast<int64_t>(a.B) * a.KH * rows;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    const int64_t at = group_index() * 8 + (threadIdx.x >> 5);
     const int d = (threadIdx.x & 31) * 4;
     if (at >= all || d >= a.D) return;
     const float* ml = a.part + a.splits * all * a.D;
@@ -646,7 +648,7 @@ int tile_rows(const Plan& how) { return how.few == 0 ? kManyRows : 16 * how.few;
 
 template <int DT>
 void launch(const WindowArgs& a, const Plan& how, int64_t grid, hipStream_t s) {
-    const unsigned n = static_cast<unsigned>(grid);
+    const dim3 n = grid_of(grid, kThreads);
     if (how.few == 0) k_window_many<DT><<<n, kThreads, 0, s>>>(a);
     else if (how.few == 1) k_window_few<DT, 1><<<n, kThreads, 0, s>>>(a);
     else k_window_few<DT, 2><<<n, kThreads, 0, s>>>(a);
@@ -696,7 +698,7 @@ void launch_attention_window(const bf16_t* q, const bf16_t* k, const bf16_t* v, 
     launch_check("attention_window");
     if (how.splits > 1) {
         const int64_t all = rows * sh.batch * sh.kv_heads;
-        k_window_join<<<static_cast<unsigned>((all + 7) / 8), kThreads, 0, s>>>(a);
+        k_window_join<<<grid_of((all + 7) / 8, kThreads), kThreads, 0, s>>>(a);
         launch_check("attention_window");
     }
 }

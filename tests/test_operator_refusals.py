@@ -95,3 +95,7 @@ def test_empty_calls_are_no_ops():
     assert lib.bh_gemm_fp8(None, None, None, None, None, None, 0, 4, 4, 0, bh.BF16, None, 0, None) == 0
     assert lib.bh_attention_window(None, 512, None, None, 128, None, 512, 0, 8, 2, 1, 4, 64, 0.0, -1, 0, 0, None, None,
                                    bh.BF16, None, 0, None) == 0
+
+
+def test_quantize_refuses_more_workgroups_than_it_numbers():
+    assert "too large" in quantize(rows=(1 << 30) - 1, cols=1 << 20, ld=1 << 20)
