@@ -189,28 +189,6 @@ struct Geom {
     static_assert(kSB >= 2 && wait(false) < 63 && kItems <= 2 * MT * NP, "LDS, vmcnt, multiply()");
 };
 
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-// gk::dma16 with a uniform base and a 32-bit offset a lane; dma4 moves four bytes a lane.
-// The wait states: one behind m0, five behind a vector instruction that wrote `base` (a register brought back from
-// where the compiler had put it), which it does not count for inline assembly.
-__device__ __forceinline__ uint32_t lds_address(const char* p) {
-    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(p)));
-}
-__device__ __forceinline__ void dma16_at(const void* base, uint32_t off, const char* lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(lds_address(lds)), "v"(off), "s"(base)
-                 : "memory", "m0");
-}
-__device__ __forceinline__ void dma4_at(const void* base, uint32_t off, const char* lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2"
-                 :
-                 : "s"(lds_address(lds)), "v"(off), "s"(base)
-                 : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
 template <int MT, int NP>
 __device__ __forceinline__ void tile_at(int v, int tiles_m, int tiles_n, int group_m, int64_t& m0, int64_t& n0) {
     const int T = tiles_m * tiles_n;

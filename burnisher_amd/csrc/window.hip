@@ -60,23 +60,6 @@ __device__ __forceinline__ int clamp_to(int64_t v, int lo, int hi) {
     return static_cast<int>(min(max(v, static_cast<int64_t>(lo)), static_cast<int64_t>(hi)));
 }
 
-__device__ __forceinline__ uint32_t lds_address(const char* p) {
-    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(p)));
-}
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-// Lane L's 16 bytes at base + off land at LDS address lds + 16 L (`base` and `lds` uniform). Inline assembly so
-// that the compiler does not wait for these loads by itself: s_waitcnt below covers them.
-// The wait states: one behind m0, five behind a vector instruction that wrote `base` (a register brought back from
-// where the compiler had put it), which it does not count for inline assembly.
-__device__ __forceinline__ void dma16(const void* base, uint32_t off, const char* lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(lds_address(lds)), "v"(off), "s"(base)
-                 : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
 // Four keys of column (lane % 16): lane i of a 16-lane group passes the address of columns 4 (i % 4) .. + 3 of the
 // group's key i / 4.
 __device__ __forceinline__ s16x4_t read_transposed(const char* p) {
@@ -329,28 +312,28 @@ __global__ void __launch_bounds__(kThreads, 2) k_window_many(WindowArgs a) {
 #pragma unroll
             for (int i = 0; i < kItems; ++i) {
                 const int n = i * 4 + wave;
-                if (i * 4 + 3 < KP + VP || n < KP + VP) dma16(n < KP ? k : v, off[i], (n < KP ? kl : vl) + n * 1024);
+                if (i * 4 + 3 < KP + VP || n < KP + VP) dma16_at(n < KP ? k : v, off[i], (n < KP ? kl : vl) + n * 1024);
             }
             return;
         }
         if ((jv < 0) & k_whole) {
 #pragma unroll
             for (int i = 0; i * 4 < KP; ++i)
-                if (i * 4 + wave < KP) dma16(k, off[i], kl + (i * 4 + wave) * 1024);
+                if (i * 4 + wave < KP) dma16_at(k, off[i], kl + (i * 4 + wave) * 1024);
             return;
         }
         if (!with_k & (jv == blocks.n - 1)) {
 #pragma unroll
             for (int i = KP / 4; i < kItems; ++i) {
                 const int n = i * 4 + wave;
-                if (n >= KP && n < KP + VP) dma16(v, off_last[i - KP / 4], vl + n * 1024);
+                if (n >= KP && n < KP + VP) dma16_at(v, off_last[i - KP / 4], vl + n * 1024);
             }
             return;
         }
 #pragma unroll 1
         for (int n = with_k ? wave : KP + (wave + 3 * KP) % 4; n < (with_v ? KP + VP : KP); n += 4) {
-            if (n < KP) dma16(k, chunk_offset<KP>(n, lane, chunks, min(k_last, kKeys - 1), ld_bytes), kl + n * 1024);
-            else dma16(v, chunk_offset<VP>(n - KP, lane, chunks, min(v_last, kKeys - 1), ld_bytes), vl + n * 1024);
+            if (n < KP) dma16_at(k, chunk_offset<KP>(n, lane, chunks, min(k_last, kKeys - 1), ld_bytes), kl + n * 1024);
+            else dma16_at(v, chunk_offset<VP>(n - KP, lane, chunks, min(v_last, kKeys - 1), ld_bytes), vl + n * 1024);
         }
     };
     auto join = [&]() {   // this wave's loads have landed and its reads are done; behind the barrier everyone's
@@ -470,12 +453,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_window_few(WindowArgs a) {
         char* to = own + slot * kStage;
         if (last >= kPiece - 1) {
 #pragma unroll
-            for (int i = 0; i < kItems; ++i) dma16(i < kK ? k : v, off[i], to + i * 1024);
+            for (int i = 0; i < kItems; ++i) dma16_at(i < kK ? k : v, off[i], to + i * 1024);
             return;
         }
 #pragma unroll 1
         for (int i = 0; i < kItems; ++i)
-            dma16(i < kK ? k : v, i < kK ? chunk_offset<KP>(i, lane, chunks, last, ld_bytes) : chunk_offset<VP>(i - kK, lane, chunks, last, ld_bytes),
+            dma16_at(i < kK ? k : v, i < kK ? chunk_offset<KP>(i, lane, chunks, last, ld_bytes) : chunk_offset<VP>(i - kK, lane, chunks, last, ld_bytes),
                   to + i * 1024);
     };
     if (j0 < j1) load(j0, 0);
