@@ -200,12 +200,17 @@ int bh_quantize_fp8(const void* x, int64_t ld_x, void* q, float* scales, int64_t
 /* The matrix product of two matrices as bh_quantize_fp8 writes them, a with block_rows 1 [m, k] and
  * b with block_rows 128 [n, k] (a checkpoint's [out_features, in_features]):
  *   out[m, n] = epilogue(sum_j a_scales[j, m] * b_scales[n / 128, j] * (a . b over block j) + bias[n])
- * with bias and out in `dtype` and `epilogue` as in bh_gemm. Sums and scales are fp32. With a BH_F32
- * output the codes are multiplied as bf16 values, exactly; with BH_BF16 by the 8-bit matrix
- * instruction, which runs at twice the rate, adds eight neighbouring products at a time and drops of
- * each what lies below 2^-13 of the largest of the eight (measured: about 2^-13 of the result, below
- * the output's own 2^-8). a and b are 16-byte aligned and hold zeros from
- * k to the end of each row.
+ * with bias and out in `dtype` and `epilogue` as in bh_gemm. Sums and scales are fp32; a block's two
+ * scales are multiplied first. With a BH_F32 output the codes are multiplied as bf16 values, exactly.
+ * With BH_BF16 they are by the 8-bit matrix instruction, which runs at twice the rate, adds the
+ * products of eight neighbouring columns at a time and drops of each product what lies below 2^-13 of
+ * the largest of the eight (measured). What a sum loses is below 8 * 2^-13 * max |a| * max |b| of
+ * each eight, times the scales. Where the products of a row mostly add up that lies below the
+ * output's own rounding, 2^-8 of it, but a sum whose large products cancel can lose all of its
+ * value: where that matters, ask for a BH_F32 output. The sizes choose the kernel, the order of the
+ * sums and the form of the epilogue's exponential, so the last bits of a row may change with the
+ * number of rows beside it; GELU and SiLU below 2^-118 may come out as zeros.
+ * a and b are 16-byte aligned and hold zeros from k to the end of each row.
  * `workspace` is device memory of workspace_bytes, 16-byte aligned, that the call may write (partial
  * sums of a split K): bh_gemm_fp8_workspace_bytes says how much a product of these sizes uses with
  * either output type, 0 for many. NULL

@@ -342,6 +342,33 @@ def test_gemm_small_whole_numbers_are_exact(hip):
         assert torch.equal(run_gemm(a8, sa, b8, sb, None, k), want.to(torch.bfloat16))
 
 
+@pytest.mark.parametrize("m", [3, 40, 300, 2048])
+def test_gemm_whose_large_products_cancel(hip, m):
+    # of every eight columns two products are +-448 * 448 and the other six whole numbers below 2^7: an fp32 output
+    # has the exact sum, a bf16 one is off by at most what the contract lets each eight lose, 8 * 2^-13 * 448 * 448, and
+    # its rounding. In the second half of the output's columns nothing cancels and the sum keeps its relative accuracy.
+    import torch
+    n, k = 200, 384
+    g = torch.Generator(device="cuda").manual_seed(m)
+    a, b = (torch.randint(-8, 9, (rows, k), generator=g, device="cuda").float() for rows in (m, n))
+    a[:, 0::8], a[:, 1::8], b[:, 0::8], b[:, 1::8] = 448, 448, 448, -448
+    b[n // 2:, 1::8] = 448
+    want = a.double() @ b.t().double().contiguous()
+    a8, b8 = a.to(torch.float8_e4m3fn), b.to(torch.float8_e4m3fn)
+    sa, sb = torch.ones(3, m, device="cuda"), torch.ones(2, 3, device="cuda")
+    off = (run_gemm(a8, sa, b8, sb, None, k, dtype="float32").double() - want).abs()
+    # Whole numbers below 2^24 are exact in fp32. Where the products cancel any part of the sum is: at most 48 * 448^2
+    # = 9.6e6 and the small ones. Where they do not, a block's sum is (16 * 2 * 448^2 = 6.4e6) and the sum of two, but not
+    # that of all three, 1.9e7: its addition rounds by half a step, 2^-24 of it.
+    alike = slice(n // 2, n)
+    assert off[:, :n // 2].max() == 0 and (off <= 2.0 ** -24 * want.abs()).all()
+    off = (run_gemm(a8, sa, b8, sb, None, k).double() - want).abs()
+    lost = k / 8 * 8 * 2.0 ** -13 * 448 * 448
+    assert (off <= lost + 2.0 ** -8 * (want.abs() + lost)).all()
+    # each eight adds up to at least 2 * 448^2 - 6 * 64 and loses below 2^-10 * 448^2
+    assert (off[:, alike] <= (2.0 ** -11 * (1 + 2.0 ** -8) + 2.0 ** -8 * (1 + 2.0 ** -10)) * want[:, alike].abs()).all()
+
+
 @pytest.mark.parametrize("m", [2, 40, 300])
 def test_gemm_keeps_a_nan_and_an_infinite_scale_in_their_rows(hip, m):
     import torch
