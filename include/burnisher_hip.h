@@ -244,7 +244,10 @@ int bh_gemm_fp8_describe(int64_t m, int64_t n, int64_t k, int dtype, int with_wo
  * a length is taken as at least 0 and at most kv_len. A query that sees no key gives zeros, unlike
  * bh_attention, whose masked keys keep a score. Keys that no query of a batch row sees are not read
  * into any sum, whatever they hold; a NaN or infinity in a key or value that one query sees may reach
- * the queries near it. softmax(scale * q k^T) v with fp32 scores, scale <= 0 meaning 1/sqrt(head_dim).
+ * the queries near it. softmax(scale * q k^T) v, scale <= 0 meaning 1/sqrt(head_dim). Scores, their
+ * maxima and the sums are fp32; a weight, exp(score - maximum), is rounded to bf16, the matrix
+ * instruction's type, before it enters the output's sum and the denominator alike. So an output is off
+ * by up to 2^-8 of the weights' average of |v - out|, beside its own rounding to bf16.
  * Element (b, s, h, d) of q lives at q[(b * q_len + s) * ld_q + h * head_dim + d], of k and v at
  * [(b * kv_len + s) * ld_kv + h * head_dim + d] and of out with ld_out. head_dim is a multiple of 8
  * up to 128, the row strides are multiples of 8 (ld_out of 4), q, k and v 16-byte and out 8-byte
