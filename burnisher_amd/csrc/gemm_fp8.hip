@@ -369,7 +369,8 @@ __device__ __forceinline__ uint32_t swap_pair(uint32_t v) {
     return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xb1, 0xf, 0xf, true));   // quad_perm 1 0 3 2
 }
 
-// 16 bytes of a row that starts anywhere: memory takes them at the alignment of an element (8192 x 8191 x 1152 135 us, element by element 209).
+// 16 bytes of a row that starts anywhere: memory takes them at the alignment of an element (8192 x 8191 x 1152 135 us,
+// element by element 209).
 template <bool LINES, typename V, typename T>
 __device__ __forceinline__ void store16(V v, T* p) {
     typedef V Any __attribute__((aligned(sizeof(T))));
@@ -440,8 +441,8 @@ __device__ __forceinline__ void store_inside(const f32x4_t (&acc)[MT][2 * NP], c
     }
 }
 
-// A lane's 8 consecutive columns of MT rows a column pair. The bias is read before the first store: vmcnt counts loads and stores in order, so a load behind a store
-// waits until memory has taken that.
+// A lane's 8 consecutive columns of MT rows a column pair. The bias is read before the first store: vmcnt counts loads and
+// stores in order, so a load behind a store waits until memory has taken that.
 template <int MT, int NP, typename OUT>
 __device__ __forceinline__ void store(const f32x4_t (&acc)[MT][2 * NP], const Fp8Args& p, int64_t m0, int64_t n0,
                                       int wm, int wn, int lr, int hi) {

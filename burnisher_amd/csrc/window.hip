@@ -250,12 +250,13 @@ __device__ __forceinline__ bool sees_all(int base, int end, int lo1, int hi0, in
 // Two workgroups a CU (three up to head_dim 64), each with two slots in LDS for K and for V; deeper rings, tiles of 256
 // rows and 32 x 32 x 16 products were no faster. What bounds it: the vector instructions, 32 exponentials and about 75
 // others a lane and block, run beside the matrix ones only in part, and a block's loads wait for each other while they are
-// issued (600 of 3200 to 4500 cycles; put between the products they cost more registers than that). Without the
+// issued (600 of 3200 to 4500 cycles, five wait states a load among them that dma16_at no longer has; put between the
+// products they cost more registers than that). Without the
 // exponentials a call takes 8 to 15% less; finding the maximum among the output product's matrix instructions, or acting on
 // it behind the barrier, gained nothing. Which blocks a wave sees, and sees whole, are ranges found before the loop, and
 // whole blocks load without a branch a load: at head_dim 64 388 -> 340 us. Measured (2 x 16384 tokens of 16 heads, window
-// 1024 to either side): head_dim 64 340 us (780 TFLOP/s), 72 450 (its columns are computed as 80 and 96), 128 571 (930);
-// 2 x 4096 tokens of 32 / 8 heads of 128, window 1023 back, 163 to 178; 2 x 300 of 64 heads of 64, 128 either side, 15.
+// 1024 to either side): head_dim 64 339 us (780 TFLOP/s), 72 445 (its columns are computed as 80 and 96), 128 576 (930);
+// 2 x 4096 tokens of 32 / 8 heads of 128, window 1023 back, 158 to 178; 2 x 300 of 64 heads of 64, 128 either side, 15.
 
 constexpr int kKeys = 64, kManyRows = 128;
 
@@ -411,8 +412,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_window_many(WindowArgs a) {
 // Bound by the keys' bytes: a wave waits only for its own loads, two pieces in flight, and the waves' sums meet
 // at the end. With `splits` the keys go to several workgroups, whose partial results k_window_join sums (4.8 us for
 // 512 rows of 128 in two splits: a launch). 16 sequences of one token, 32 / 8 heads of 128, window 4095 back in up
-// to 8192 keys: 54 us with the join, 5.0 TB/s. 4 x 64 tokens of the same heads, on 32-row tiles: 52 us (56 with a branch a
-// load for the pieces that end inside).
+// to 8192 keys: 54 us with the join, 5.0 TB/s. 4 x 64 tokens of the same heads, on 32-row tiles: 46 us (52 when each load
+// waited for its base).
 
 constexpr int kPiece = 32;
 
@@ -579,16 +580,17 @@ int device_cus() {
 }
 
 // How a call runs: k_window_many, or k_window_few on tiles of 16 `few` rows with the keys in `splits`. The estimates, in
-// us, were checked on 35 shapes on one MI355X (head_dim 32 to 128, 1 to 2048 rows of 77 to 16000 keys), each on every
-// kernel and split that fits it: what they choose is within 5% of the fastest. Beside 3.5 a workgroup,
+// us, were checked on 30 shapes on one MI355X (head_dim 32 to 128, 4 to 16384 rows of 77 to 16384 keys), each on every
+// kernel and split that fits it: what they choose is within 6% of the fastest on 27, and 9 to 13% above it on 8 x 4 tokens
+// of 16 / 4 heads against 3000 keys (eight splits 13.4 to 17.5, four 12.0 to 16.0). Beside 3.5 a workgroup,
 //  - many: a block of 64 keys costs 0.62 + 0.006 head_dim alone on a CU, 0.5 + 0.014 beside another workgroup;
 //  - few: a piece of 32 keys for each of the four waves costs 0.35 + 0.005 head_dim on 16 rows and 0.3 + 0.009 on 32, one
 //    workgroup a CU (two up to head_dim 64), and no less in all than reading the keys at
 //    5.2 TB/s (a quarter more on fewer workgroups than CUs);
 //  - a join costs 3 + 0.25 a split and its partial results at 3 TB/s.
-// 16 sequences of a token each, 32 / 8 heads of 128, 4096 keys: two splits 57 us, none 65, k_window_many 90. Four times
-// 64 tokens of the same: 32-row tiles 52, 16-row 82, k_window_many 88. 2 x 64 heads of 300 tokens, head_dim 64:
-// k_window_many 15.5, 32-row tiles 24. (64-row tiles were never ahead of these, 55 and 33 there.)
+// 16 sequences of a token each, 32 / 8 heads of 128, 4096 keys: two splits 58 us, none 64, k_window_many 87. Four times
+// 64 tokens of the same: 32-row tiles 46, 16-row 63, k_window_many 83. 2 x 64 heads of 300 tokens, head_dim 64:
+// k_window_many 14.8, 32-row tiles 23. (64-row tiles were never ahead of these.)
 struct Plan {
     int few;      // 0: k_window_many
     int splits;

@@ -213,7 +213,7 @@ def test_gemm_sizes(hip, m, n, k, dtype):
     check_gemm(m, n, k, dtype=dtype)
 
 
-# one and several blocks of K, one and several tiles a workgroup, K whole and in slices, on every tile
+# one and several blocks of K, few and many tiles; test_gpu_fp8_variants.py reaches every form
 TILE_SIZES = [(454, 3853, 16), (33, 39, 5011), (817, 4616, 170), (272, 3733, 3941), (929, 1287, 2911), (1843, 4127, 330),
               (521, 3680, 4188), (2763, 2222, 200), (404, 4285, 5927), (1592, 802, 5735), (2256, 3619, 330),
               (2951, 3411, 16), (2875, 4239, 330), (4500, 4300, 160), (2048, 2048, 2048)]

@@ -122,7 +122,7 @@ def test_head_dims_of_many_rows(hip, d):
     check(8, 16, 16, 70, 90, d, 20, 5, 3, lens=[90, 89, 70, 64, 33, 90, 90, 12], starts=[20, 0, 0, 10, 3, -5, 40, 0])
 
 
-# tiles of 16, 32, 64 and 128 rows, the keys whole and split, at every width
+# few and many rows against few and many keys, at every width of the kernels' images
 @pytest.mark.parametrize("d", [24, 64, 72, 88, 128])
 @pytest.mark.parametrize("heads,kvh,n,kv_len,left,right,sinks", [
     (4, 4, 4, 1500, -1, 0, 0), (40, 8, 33, 300, 300, 300, 0), (40, 8, 70, 300, -1, 0, 0), (8, 8, 33, 1500, -1, 0, 0),
