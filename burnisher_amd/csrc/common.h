@@ -156,9 +156,10 @@ inline void require(bool ok, const std::string& msg) {
 // ---- launches of any number of workgroups ------------------------------------------------------
 
 // A launch has fewer than 2^32 threads along an axis (2^24 workgroups of 256), so what is beyond goes on along y. The
-// kernel takes its number from group_index(); numbers from `groups` on, in the last row, have nothing to do.
+// kernel takes its number from group_index(); numbers from `groups` on, in the last row, have nothing to do (and may pass
+// 2^31 where `groups` does not).
 inline dim3 grid_of(int64_t groups, int threads) {
-    const int64_t most = ((int64_t{1} << 32) - 1) / threads, y = (groups + most - 1) / most;
+    const int64_t most = ((int64_t{1} << 32) - 1) / threads, y = 1 + (groups - 1) / most;
     return dim3(static_cast<unsigned>((groups + y - 1) / y), static_cast<unsigned>(y));
 }
 __device__ __forceinline__ int64_t group_index() { return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }

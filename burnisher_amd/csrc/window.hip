@@ -268,8 +268,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_window_many(WindowArgs a) {
     __shared__ __attribute__((aligned(1024))) char kmem[2 * kKBytes], vmem[2 * kVBytes];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int T = a.tiles * a.B * a.KH;
-    int id = static_cast<int>(group_index());
-    if (id >= T) return;
+    const int64_t number = group_index();
+    if (number >= T) return;
+    int id = static_cast<int>(number);
     if ((T & 7) == 0) id = (id & 7) * (T >> 3) + (id >> 3);   // neighbouring tiles, which share keys, on one XCD
     const int tile = id % a.tiles, bk = id / a.tiles, kh = bk % a.KH, b = bk / a.KH;
     const int rows = a.group * a.Sq, row0 = tile * kManyRows, row1 = min(row0 + kManyRows, rows) - 1;
@@ -426,8 +427,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_window_few(WindowArgs a) {
     __shared__ __attribute__((aligned(1024))) char smem[4 * 2 * kStage];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int T = a.tiles * a.splits * a.B * a.KH;
-    int id = static_cast<int>(group_index());
-    if (id >= T) return;
+    const int64_t number = group_index();
+    if (number >= T) return;
+    int id = static_cast<int>(number);
     if ((T & 7) == 0) id = (id & 7) * (T >> 3) + (id >> 3);   // tiles that read the same keys on one XCD
     const int tile = id % a.tiles, split = id / a.tiles % a.splits, bk = id / a.tiles / a.splits, kh = bk % a.KH, b = bk / a.KH;
     const int rows = a.group * a.Sq, row0 = tile * (16 * QT), row1 = min(row0 + 16 * QT, rows) - 1;

@@ -52,5 +52,12 @@ def test_memory_instructions_wait_for_a_scalar_address(path):
     assert all(n is None or n >= 5 for n in waits_for_scalar_addresses((CSRC / path).read_text()))
 
 
+@pytest.mark.parametrize("path", sorted(p.name for p in CSRC.iterdir()))
+def test_workgroup_numbers_are_compared_before_they_are_narrowed(path):
+    # the last row of a launch along y may count past 2^31
+    assert not re.search(r"(static_cast<(unsigned|int|u?int32_t)>|\(int\)|\bint \w+ = |\bunsigned \w+ = )\s*\(?group_index\(\)",
+                         (CSRC / path).read_text())
+
+
 def test_direct_loads_with_a_scalar_address_are_found():
     assert len(waits_for_scalar_addresses((CSRC / "common.h").read_text())) == 2
