@@ -22,6 +22,7 @@ ST_DTYPES = {ST_F32: "F32", ST_BF16: "BF16", ST_F16: "F16", ST_F8_E4M3: "F8_E4M3
 EPI_NONE, EPI_GELU, EPI_SILU, EPI_GELU_GATED = 0, 1, 2, 3
 DIT_FUSED, DIT_OPWISE = 0, 1
 ROWS_JOINED, ROWS_SPLIT = 0, 1
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
 (K_GEMM, K_GEMV, K_ATTN_SELF, K_ATTN_CROSS, K_NORM, K_ELEMENTWISE, K_GEMM_FF0, K_GEMM_FF2,
  K_GEMM_QKV) = range(9)
 KERNEL_CLASSES = ["gemm", "gemv", "attention_self", "attention_cross", "norm", "elementwise",
@@ -106,6 +107,33 @@ class AttentionWindowPlan(ctypes.Structure):
     _fields_ = [("tile_rows", ctypes.c_int), ("splits", ctypes.c_int), ("workgroups", ctypes.c_int64)]
 
 
+class RopeAxes(ctypes.Structure):
+    _fields_ = [("axes", ctypes.c_int), ("pairs", ctypes.c_int * 4), ("theta", ctypes.c_double),
+                ("scale", ctypes.c_double * 4), ("joint", ctypes.c_int), ("interleaved", ctypes.c_int)]
+
+    @classmethod
+    def of(cls, pairs, theta: float = 10000.0, scale=(), joint: bool = False, interleaved: bool = False) -> "RopeAxes":
+        """`pairs` of columns for each axis; positions multiplied by `scale` (1 for axes that it does not name)."""
+        if not 1 <= len(pairs) <= 4 or len(scale) > len(pairs):
+            raise BurnisherError(f"rope: 1 to 4 axes and at most a scale for each, not {len(pairs)} and {len(scale)}")
+        padded = [*scale, *[1.0] * (4 - len(scale))]
+        return cls(axes=len(pairs), pairs=(ctypes.c_int * 4)(*pairs), theta=theta, scale=(ctypes.c_double * 4)(*padded),
+                   joint=int(joint), interleaved=int(interleaved))
+
+
+class AttentionLinearPlan(ctypes.Structure):
+    _fields_ = [("chunk", ctypes.c_int), ("segments", ctypes.c_int), ("workgroups", ctypes.c_int64)]
+
+
+class ResidualNorms(ctypes.Structure):
+    _fields_ = [("post_norm", ctypes.c_int), ("post_weight", ctypes.c_void_p), ("post_bias", ctypes.c_void_p),
+                ("post_eps", ctypes.c_float), ("gate", ctypes.c_void_p), ("branch_scale", ctypes.c_float),
+                ("residual_scale", ctypes.c_float), ("pre_norm", ctypes.c_int), ("pre_weight", ctypes.c_void_p),
+                ("pre_bias", ctypes.c_void_p), ("pre_eps", ctypes.c_float), ("scale", ctypes.c_void_p),
+                ("shift", ctypes.c_void_p), ("mod_rows", ctypes.c_int64), ("ld_mod", ctypes.c_int64),
+                ("weight_offset", ctypes.c_float)]
+
+
 class SchedCoefficients(ctypes.Structure):
     _fields_ = [("order", ctypes.c_int)] + [
         (f, ctypes.c_double) for f in ("sigma_s0", "sigma_t", "sigma_vp_s0", "sigma_vp_t",
@@ -152,6 +180,14 @@ SIGNATURES = {
                              _I64, _I64, _V, _V, _I, _V, _I64, _V], _I),
     "bh_attention_window_workspace_bytes": ([_I64] * 9, _I64),
     "bh_attention_window_describe": ([_I64] * 9 + [_I, _I, ctypes.POINTER(AttentionWindowPlan)], _I),
+    "bh_rope": ([ctypes.POINTER(RopeAxes), _V, _I64, _V, _I64, _V, _I64, _I64, _V, _I64, _V, _I64, _I64, _I64,
+                 _I64, _I, _I, _V], _I),
+    "bh_attention_linear": ([_V, _I64, _V, _I64, _V, _I64, _V, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _V,
+                             _V, _V, _V, _I, _V, _I64, _V], _I),
+    "bh_attention_linear_workspace_bytes": ([_I64] * 6, _I64),
+    "bh_attention_linear_describe": ([_I64] * 6 + [_I, _I, ctypes.POINTER(AttentionLinearPlan)], _I),
+    "bh_residual_norms_run": ([_V, _I64, _V, _I64, _V, _I64, _V, _I64, _I64, _I64, ctypes.POINTER(ResidualNorms),
+                               _I, _I, _V], _I),
     "bh_scale": ([_V, _V, _I64, _F, _I, _V], _I),
     "bh_timestep_embedding": ([_D, _I, _I64, _V, _I, _V], _I),
     "bh_probe_device": ([_V, _V, _I64, ctypes.POINTER(ProbeResult)], _I),

@@ -516,6 +516,183 @@ int bh_attention_window(const void* q, int64_t ld_q, const void* k, const void* 
     });
 }
 
+int bh_rope(const bh_rope_axes* axes, const int32_t* positions, int64_t position_rows, const void* q,
+            int64_t ld_q, void* q_out, int64_t ld_q_out, int64_t q_heads, const void* k, int64_t ld_k,
+            void* k_out, int64_t ld_k_out, int64_t k_heads, int64_t rows, int64_t head_dim, int inverse,
+            int dtype, void* stream) {
+    return guarded([&] {
+        const char* op = "rope (hip-gfx950)";
+        const bool f32 = is_f32(dtype);
+        require(axes != nullptr, "rope: axes is null");
+        require(axes->axes >= 1 && axes->axes <= 4, "rope: 1 to 4 axes");
+        int64_t pairs = 0;
+        for (int a = 0; a < axes->axes; ++a) {
+            require(axes->pairs[a] >= 0, "rope: an axis turns a negative number of pairs");
+            require(std::isfinite(axes->scale[a]), "rope: a scale is not finite");
+            pairs += axes->pairs[a];
+        }
+        require(pairs >= 1 && pairs <= kRopePairs, "rope: the axes turn 1 to 128 pairs in all");
+        require(std::isfinite(axes->theta) && axes->theta > 0.0, "rope: theta must be finite and above 0");
+        require_nonneg(rows, op, "rows");
+        require_nonneg(q_heads, op, "q_heads");
+        require_nonneg(k_heads, op, "k_heads");
+        require(head_dim >= 2 * pairs && head_dim <= 1024, "rope: head_dim must hold the turned pairs and be at most 1024");
+        require(q_heads < 65536 && k_heads < 65536 && q_heads + k_heads < 65536, "rope: fewer than 2^16 heads in all");
+        require(rows < (int64_t{1} << 40), "rope: rows must be below 2^40");
+        require(ld_q >= q_heads * head_dim && ld_q_out >= q_heads * head_dim && ld_k >= k_heads * head_dim &&
+                    ld_k_out >= k_heads * head_dim,
+                "rope: a row stride is below its heads * head_dim");
+        if (rows == 0 || q_heads + k_heads == 0) return;
+        require(position_rows >= 1, "rope: position_rows must be positive");
+        require_device_ptr(positions, op, "positions");
+        const uintptr_t size = f32 ? 4 : 2;
+        bool fits = aligned(positions, 4);
+        if (q_heads) {
+            require_device_ptr(q, op, "q");
+            require_device_ptr(q_out, op, "q_out");
+            fits = fits && aligned(q, size) && aligned(q_out, size);
+            require(q != q_out || ld_q == ld_q_out, "rope: q_out is q with another stride");
+        }
+        if (k_heads) {
+            require_device_ptr(k, op, "k");
+            require_device_ptr(k_out, op, "k_out");
+            fits = fits && aligned(k, size) && aligned(k_out, size);
+            require(k != k_out || ld_k == ld_k_out, "rope: k_out is k with another stride");
+        }
+        require(fits, "rope: an operand is not aligned to its type");
+        ProfileScope ps(K_ELEMENTWISE, as_stream(stream), 2.0 * rows * (q_heads + k_heads) * head_dim * size);
+        launch_rope(*axes, positions, position_rows, RopeSide{q, q_out, ld_q, ld_q_out, static_cast<int>(q_heads)},
+                    RopeSide{k, k_out, ld_k, ld_k_out, static_cast<int>(k_heads)}, rows, head_dim, inverse != 0, f32,
+                    as_stream(stream));
+    });
+}
+
+namespace {
+LinearShape linear_shape(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len, int64_t head_dim,
+                         int64_t value_dim) {
+    const char* op = "attention_linear (hip-gfx950)";
+    require_nonneg(batch, op, "batch");
+    require_nonneg(heads, op, "heads");
+    require_nonneg(seq_len, op, "seq_len");
+    require(kv_heads > 0 && heads % kv_heads == 0, "attention_linear: heads must be a multiple of kv_heads");
+    require(head_dim > 0 && head_dim <= 128 && head_dim % 8 == 0 && value_dim > 0 && value_dim <= 128 && value_dim % 8 == 0,
+            "attention_linear (hip-gfx950): head_dim and value_dim must be multiples of 8 up to 128");
+    require(batch < kSizeLimit && heads < kSizeLimit && seq_len < kSizeLimit, "attention_linear: seq_len must be below 2^30");
+    require(batch * heads < (int64_t{1} << 31), "attention_linear: batch * heads must be below 2^31");
+    return LinearShape{batch, heads, kv_heads, seq_len, head_dim, value_dim, 0, 0, 0, 0, 0.f};
+}
+}  // namespace
+
+int64_t bh_attention_linear_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len,
+                                            int64_t head_dim, int64_t value_dim) {
+    int64_t bytes = -1;
+    (void)guarded([&] {
+        const LinearShape sh = linear_shape(batch, heads, kv_heads, seq_len, head_dim, value_dim);
+        bytes = batch * heads * seq_len == 0 ? 0 : 4 * attention_linear_workspace_floats(sh);
+    });
+    return bytes;
+}
+
+int bh_attention_linear_describe(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len, int64_t head_dim,
+                                 int64_t value_dim, int with_workspace, int cus, bh_attention_linear_plan* out) {
+    return guarded([&] {
+        const LinearShape sh = linear_shape(batch, heads, kv_heads, seq_len, head_dim, value_dim);
+        require(cus >= 0, "attention_linear_describe: cus is negative");
+        require(out != nullptr, "attention_linear_describe: out is null");
+        *out = batch * heads * seq_len == 0 ? bh_attention_linear_plan{} : attention_linear_plan(sh, with_workspace != 0, cus);
+    });
+}
+
+int bh_attention_linear(const void* q, int64_t ld_q, const void* k, int64_t ld_k, const void* v, int64_t ld_v,
+                        void* out, int64_t ld_out, int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len,
+                        int64_t head_dim, int64_t value_dim, float scale, const float* log_decay, const int32_t* lens,
+                        const float* state_in, float* state_out, int dtype, void* workspace, int64_t workspace_bytes,
+                        void* stream) {
+    return guarded([&] {
+        const char* op = "attention_linear (hip-gfx950)";
+        require(!is_f32(dtype), "attention_linear (hip-gfx950): bf16 only");
+        LinearShape sh = linear_shape(batch, heads, kv_heads, seq_len, head_dim, value_dim);
+        require(ld_q >= heads * head_dim && ld_k >= kv_heads * head_dim && ld_v >= kv_heads * value_dim &&
+                    ld_out >= heads * value_dim,
+                "attention_linear: a row stride is below its heads * head_dim");
+        require(ld_q % 8 == 0 && ld_k % 8 == 0 && ld_v % 8 == 0 && ld_out % 4 == 0,
+                "attention_linear: ld_q, ld_k and ld_v must be multiples of 8, ld_out of 4");
+        const int64_t most = int64_t{1} << 24;
+        require(ld_q < most && ld_k < most && ld_v < most, "attention_linear: ld_q, ld_k and ld_v must be below 2^24");
+        if (batch * heads == 0 || (seq_len == 0 && !state_out)) return;
+        if (seq_len > 0) {   // without tokens the state is copied
+            require_device_ptr(q, op, "q");
+            require_device_ptr(k, op, "k");
+            require_device_ptr(v, op, "v");
+            require_device_ptr(out, op, "out");
+        }
+        require_device_ptr(log_decay, op, "log_decay");
+        optional_device_ptr(lens, op, "lens");
+        optional_device_ptr(state_in, op, "state_in");
+        optional_device_ptr(state_out, op, "state_out");
+        require(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 8),
+                "attention_linear: q, k and v must be 16-byte, out 8-byte aligned");
+        require(aligned(state_in, 16) && aligned(state_out, 16), "attention_linear: a state is not 16-byte aligned");
+        require(aligned(log_decay, 4) && aligned(lens, 4), "attention_linear: an operand is not aligned to its type");
+        sh.ld_q = ld_q;
+        sh.ld_k = ld_k;
+        sh.ld_v = ld_v;
+        sh.ld_o = ld_out;
+        sh.scale = scale > 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(head_dim));
+        const int64_t need = 4 * attention_linear_workspace_floats(sh);
+        float* ws = checked_workspace(workspace, workspace_bytes, need, "attention_linear");
+        launch_attention_linear(static_cast<const bf16_t*>(q), static_cast<const bf16_t*>(k), static_cast<const bf16_t*>(v),
+                                static_cast<bf16_t*>(out), sh, log_decay, lens, state_in, state_out, ws, as_stream(stream));
+    });
+}
+
+int bh_residual_norms_run(const void* x, int64_t ld_x, const void* residual, int64_t ld_residual, void* residual_out,
+                          int64_t ld_residual_out, void* out, int64_t ld_out, int64_t rows, int64_t cols,
+                          const bh_residual_norms* f, int residual_dtype, int dtype, void* stream) {
+    return guarded([&] {
+        const char* op = "residual_norms (hip-gfx950)";
+        const bool f32 = is_f32(dtype), res_f32 = is_f32(residual_dtype);
+        require(res_f32 || !f32, "residual_norms: a bf16 residual needs bf16 operands");
+        require_nonneg(rows, op, "rows");
+        require(cols > 0 && cols <= kResidualNormsCols, "residual_norms: cols must be 1 to 32768");
+        require(f != nullptr, "residual_norms: the struct is null");
+        auto known = [](int kind) { return kind == BH_NORM_NONE || kind == BH_NORM_LAYER || kind == BH_NORM_RMS; };
+        require(known(f->post_norm) && known(f->pre_norm), "residual_norms: unknown norm");
+        require(f->post_norm != BH_NORM_NONE || (!f->post_weight && !f->post_bias),
+                "residual_norms: post_weight or post_bias without a norm");
+        require(f->pre_norm != BH_NORM_NONE || (!f->pre_weight && !f->pre_bias),
+                "residual_norms: pre_weight or pre_bias without a norm");
+        require(f->post_eps >= 0.0f && f->pre_eps >= 0.0f, "residual_norms: eps is negative");
+        require(out || residual_out, "residual_norms: neither out nor residual_out is wanted");
+        require(ld_x >= cols && ld_residual >= cols && (!out || ld_out >= cols) && (!residual_out || ld_residual_out >= cols),
+                "residual_norms: a row stride is below cols");
+        if (rows == 0) return;
+        require_device_ptr(x, op, "x");
+        require_device_ptr(residual, op, "residual");
+        optional_device_ptr(residual_out, op, "residual_out");
+        optional_device_ptr(out, op, "out");
+        require(residual_out != residual || ld_residual_out == ld_residual, "residual_norms: residual_out is residual with another stride");
+        require(out != x || ld_out == ld_x, "residual_norms: out is x with another stride");
+        const uintptr_t size = f32 ? 4 : 2;
+        bool fits = aligned(x, size) && aligned(out, size) && aligned(residual, res_f32 ? 4 : 2) && aligned(residual_out, res_f32 ? 4 : 2);
+        const std::pair<const void*, const char*> rest[] = {
+            {f->post_weight, "post_weight"}, {f->post_bias, "post_bias"}, {f->gate, "gate"}, {f->pre_weight, "pre_weight"},
+            {f->pre_bias, "pre_bias"},       {f->scale, "scale"},         {f->shift, "shift"}};
+        for (const auto& [p, name] : rest) {
+            optional_device_ptr(p, op, name);
+            fits = fits && aligned(p, size);
+        }
+        require(fits, "residual_norms: an operand is not aligned to its type");
+        if (f->gate || f->scale || f->shift) {
+            require(f->mod_rows >= 1, "residual_norms: mod_rows must be positive");
+            require(f->ld_mod >= cols || f->mod_rows >= rows, "residual_norms: ld_mod is below cols");
+        }
+        ProfileScope ps(K_NORM, as_stream(stream), 2.0 * rows * cols * (size + (res_f32 ? 4 : 2)));
+        launch_residual_norms(x, ld_x, residual, ld_residual, residual_out, ld_residual_out, out, ld_out, rows, cols, *f,
+                              res_f32, f32, as_stream(stream));
+    });
+}
+
 int bh_gather(const void* table, const float* ids, void* out, int64_t rows, int64_t cols,
               int64_t table_rows, int dtype, void* stream) {
     return guarded([&] {

@@ -616,4 +616,30 @@ bh_attention_window_plan attention_window_plan(const WindowShape& sh, bool may_s
 void launch_attention_window(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16_t* out, const WindowShape& sh,
                              const int32_t* kv_lens, const int32_t* q_starts, float* ws, hipStream_t s);
 
+// ---- a linear-attention block (rope.hip, linear.hip, residual_norms.hip) ----
+constexpr int kRopePairs = 128;
+struct RopeSide {
+    const void* in;
+    void* out;
+    int64_t ld_in, ld_out;
+    int heads;
+};
+// Turns by positions [position_rows, axes]; the arguments have passed bh_rope's checks.
+void launch_rope(const bh_rope_axes& axes, const int32_t* positions, int64_t position_rows, const RopeSide& q, const RopeSide& k,
+                 int64_t rows, int64_t head_dim, bool inverse, bool f32, hipStream_t s);
+struct LinearShape {
+    int64_t batch, heads, kv_heads, seq_len, head_dim, value_dim;
+    int64_t ld_q, ld_k, ld_v, ld_o;   // row strides in elements
+    float scale;                      // resolved (never <= 0)
+};
+int64_t attention_linear_workspace_floats(const LinearShape& sh);
+bh_attention_linear_plan attention_linear_plan(const LinearShape& sh, bool may_split, int cus);
+void launch_attention_linear(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16_t* out, const LinearShape& sh,
+                             const float* log_decay, const int32_t* lens, const float* state_in, float* state_out, float* ws,
+                             hipStream_t s);
+constexpr int64_t kResidualNormsCols = 32768;
+void launch_residual_norms(const void* x, int64_t ld_x, const void* residual, int64_t ld_res, void* residual_out,
+                           int64_t ld_res_out, void* out, int64_t ld_out, int64_t rows, int64_t cols,
+                           const bh_residual_norms& f, bool residual_f32, bool f32, hipStream_t s);
+
 }  // namespace bh

@@ -14,6 +14,7 @@
 // rows of a 600 x 10240 bf16 matrix 6.0 us, 18.8 MB at 3.1 TB/s, of which a launch is 3.5; one row of 4096
 // 5.2 us, the call itself.
 #include "common.h"
+#include "vec8.h"
 
 #include <algorithm>
 
@@ -23,39 +24,6 @@ namespace {
 constexpr float kE4m3Max = 448.0f;
 constexpr uint32_t kAmaxFloorBits = 0x0f800000u;   // 2^-96
 constexpr int kThreads = 256;
-
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ float value(float v) { return v; }
-__device__ __forceinline__ float value(bf16_t v) { return bf2f(v); }
-
-// Eight values at column `col` of a row (its address `p` is that of `col`), zero from column `cols` on. Memory takes 16 bytes
-// at the alignment of a value, so rows of any stride load alike (8192 x 4607 bf16: 27 us, value by value 52).
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int64_t col, int64_t cols, float (&v)[8]) {
-    if (col + 8 <= cols) {
-        if constexpr (sizeof(T) == 2) {
-            typedef u32x4_t Any __attribute__((aligned(2)));
-            const u32x4_t w = *reinterpret_cast<const Any*>(p);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
-        } else {
-            typedef f32x4_t Any __attribute__((aligned(4)));
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const f32x4_t r = *reinterpret_cast<const Any*>(p + 4 * i);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * i + e] = r[e];
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = col + e < cols ? value(p[e]) : 0.0f;
-}
 
 // The magnitudes' largest bit pattern of eight values (NaN above infinity above the finite ones).
 __device__ __forceinline__ uint32_t amax8(const float (&v)[8]) {

@@ -274,6 +274,110 @@ int bh_attention_window_describe(int64_t batch, int64_t heads, int64_t kv_heads,
                                  int64_t head_dim, int64_t window_left, int64_t window_right, int64_t sinks,
                                  int with_workspace, int cus, bh_attention_window_plan* out);
 
+/* ---- a linear-attention block: rotary positions, attention with a decay, norms around the residual -- */
+
+/* Rotary positions with up to four axes (a text position; row and column of an image; time, height and
+ * width of a video). Each axis turns pairs of columns of a head: pair i, columns (u, v), becomes
+ *   (u cos t - v sin t, u sin t + v cos t),  t = position on the pair's axis * scale[axis] * frequency.
+ * The pairs are numbered axis by axis, pairs[0] of the first axis first. The angles are computed in fp64
+ * and reduced to one turn before their sine and cosine are taken in fp32, so far positions keep theirs. */
+typedef struct bh_rope_axes {
+    int axes;            /* 1 to 4 */
+    int pairs[4];        /* pairs of columns that each axis turns; at most 128 in all */
+    double theta;        /* the frequencies' base, above 0 */
+    double scale[4];     /* positions are multiplied by it (1: as they are) */
+    int joint;           /* 0: pair j of an axis turns by theta^(-j / pairs[axis]); 1: pair i of all by theta^(-i / all) */
+    int interleaved;     /* 1: pair i is columns 2i and 2i + 1; 0: columns i and (all pairs) + i */
+} bh_rope_axes;
+
+/* Turns q [rows, q_heads, head_dim] and k [rows, k_heads, head_dim] (either with no heads: not), rows ld_*
+ * elements apart, into q_out and k_out; columns behind the turned ones are copied. `positions` is int32
+ * [position_rows, axes] on the device; row r stands at positions[r % position_rows], so batch rows can
+ * share a grid's. With `inverse` everything turns back, which is also the gradient of turning. An output may
+ * be its input, with the same stride, and must not overlap one otherwise. bf16 or fp32, of any alignment of
+ * its type; rows below 2^40, head_dim at most 1024, fewer than 2^16 heads in all. The reference has no
+ * counterpart. */
+int bh_rope(const bh_rope_axes* axes, const int32_t* positions, int64_t position_rows, const void* q,
+            int64_t ld_q, void* q_out, int64_t ld_q_out, int64_t q_heads, const void* k, int64_t ld_k,
+            void* k_out, int64_t ld_k_out, int64_t k_heads, int64_t rows, int64_t head_dim, int inverse,
+            int dtype, void* stream);
+
+/* Causal linear attention with a decay for each key head, over grouped heads; bf16 with fp32 states. Query
+ * head h reads key head h / (heads / kv_heads). For each batch row and key head, over its tokens t:
+ *   S_t = exp(log_decay) * S_{t-1} + k_t (outer) v_t      a [head_dim, value_dim] matrix
+ *   out_t = scale * q_t . S_t
+ * from S before the first token in state_in (NULL: zeros) to S behind the last one in state_out (NULL: not
+ * wanted), both fp32 [batch, kv_heads, head_dim, value_dim]; state_out may be state_in and must not overlap
+ * it otherwise. One token against a state and a long prompt are the same call: sizes choose between a kernel
+ * that takes token after token and one of chunks, whose sequence is split where there are few heads.
+ * `log_decay` is fp32 [kv_heads] on the device; a value above 0, or NaN, counts as 0 (no decay), and -infinity
+ * forgets everything but the token itself. `lens` (NULL: seq_len) is int32 [batch] on the device, taken as at
+ * least 0 and at most seq_len: a sequence ends there, nothing behind it is read and its outputs are zeros.
+ * scale <= 0 means 1/sqrt(head_dim). Scores, states and sums are fp32; where they are factors of a matrix
+ * product they are sums of two or three bf16 terms (16 bits and more of a score or state that enters an
+ * output, 24 of what enters a state), so a bf16 output is off by its own rounding and little else. An infinity or NaN
+ * in a key or value reaches the outputs and the state behind it and may reach those of the 31 tokens before
+ * it. Element (b, s, h, d) of q lives at
+ * q[(b * seq_len + s) * ld_q + h * head_dim + d], likewise k, and v and out with value_dim. head_dim and
+ * value_dim are multiples of 8 up to 128, the row strides multiples of 8 (ld_out of 4) and ld_q, ld_k and
+ * ld_v below 2^24, q, k and v 16-byte, out 8-byte and the states 16-byte aligned, seq_len below 2^30 and
+ * batch * heads below 2^31. `workspace` as in bh_gemm_fp8: the states of a split sequence. It has no
+ * counterpart in the reference. */
+int bh_attention_linear(const void* q, int64_t ld_q, const void* k, int64_t ld_k, const void* v,
+                        int64_t ld_v, void* out, int64_t ld_out, int64_t batch, int64_t heads,
+                        int64_t kv_heads, int64_t seq_len, int64_t head_dim, int64_t value_dim,
+                        float scale, const float* log_decay, const int32_t* lens, const float* state_in,
+                        float* state_out, int dtype, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+int64_t bh_attention_linear_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
+                                            int64_t seq_len, int64_t head_dim, int64_t value_dim);
+
+/* The same of a bh_attention_linear call, as bh_gemm_fp8_describe. */
+typedef struct bh_attention_linear_plan {
+    int chunk;            /* tokens a step takes at once; 1: token after token */
+    int segments;         /* of a sequence, side by side; above 1 the workspace takes their states */
+    int64_t workgroups;
+} bh_attention_linear_plan;
+int bh_attention_linear_describe(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len,
+                                 int64_t head_dim, int64_t value_dim, int with_workspace, int cus,
+                                 bh_attention_linear_plan* out);
+
+/* The norm of a block's output x, its gate and scale into the residual stream, and the norm before the next
+ * block, in one pass over the rows:
+ *   n = post_norm(x);  r = residual_scale * residual + branch_scale * gate[row / mod_rows] * n
+ *   residual_out = r;  out = pre_norm(r) * (1 + scale[row / mod_rows]) + shift[row / mod_rows]
+ * A norm is none, LayerNorm or RMSNorm over the row, times (weight_offset + weight) plus bias, where given:
+ *   LayerNorm (x - mean) / sqrt(var + eps), RMSNorm x / sqrt(mean(x^2) + eps)
+ * with fp32 statistics, the variance from the differences to the mean. r enters the second norm as computed,
+ * before it is rounded for residual_out. Pointers that are NULL are left out (a factor of 1, a term of 0). */
+typedef enum bh_norm_kind { BH_NORM_NONE = 0, BH_NORM_LAYER = 1, BH_NORM_RMS = 2 } bh_norm_kind;
+typedef struct bh_residual_norms {
+    int post_norm;             /* bh_norm_kind */
+    const void* post_weight;   /* [cols], as all weights and biases in `dtype` */
+    const void* post_bias;
+    float post_eps;
+    const void* gate;          /* rows of cols elements ld_mod apart, as scale and shift: one per mod_rows rows */
+    float branch_scale, residual_scale;
+    int pre_norm;
+    const void* pre_weight;
+    const void* pre_bias;
+    float pre_eps;
+    const void* scale;
+    const void* shift;
+    int64_t mod_rows, ld_mod;
+    float weight_offset;       /* 0, or 1 where weights are stored as their difference to 1 */
+} bh_residual_norms;
+
+/* x and out [rows, cols] are in `dtype`, residual and residual_out in `residual_dtype`, which is BH_F32 or
+ * `dtype` (a bf16 model may keep its stream in fp32); rows are ld_* elements apart. out or residual_out may
+ * be NULL (not wanted); residual_out may be residual and out may be x, with the same stride, and must not
+ * overlap an operand otherwise. cols at most 32768, any alignment of the type. The reference's counterpart is
+ * a sequence of norm, modulate and add (ops.h:81-143). */
+int bh_residual_norms_run(const void* x, int64_t ld_x, const void* residual, int64_t ld_residual,
+                          void* residual_out, int64_t ld_residual_out, void* out, int64_t ld_out,
+                          int64_t rows, int64_t cols, const bh_residual_norms* f, int residual_dtype,
+                          int dtype, void* stream);
+
 /* ---- device probe ---------------------------------------------------------------------------- */
 
 /* What the device sustains, measured by this library's own kernels (the reference's `probe`
