@@ -1,8 +1,24 @@
 // Causal linear attention with a decay for each key head:
 //   S_t = decay * S_{t-1} + k_t (outer) v_t,  out_t = scale * q_t . S_t.
+//
+// Tokens by the chunk of C = 32: with S the state before the chunk, i and j tokens of it,
+//   out_i = scale * (decay^(i + 1) q_i . S + sum_{j <= i} decay^(i - j) (q_i . k_j) v_j)
+//   S'    = decay^C S + sum_j decay^(C - 1 - j) k_j (outer) v_j,
+// four matrix products, all on v_mfma_f32_16x16x32_bf16. A workgroup's waves share a chunk of q, k and v in LDS and
+// each keep 16 or 32 columns of the state in accumulators for all chunks; every wave computes the chunk's
+// scores anew (12 of its 100 matrix instructions at 128 x 128). Products are formed transposed, S and out^T from V^T, so
+// that two accumulator tiles of 16 rows, of scores or state, are one operand of the next product, in an order of its
+// 32 columns (4 g + r, then 16 + 4 g + r for lane group g) that the other operand's loads follow.
+//
+// Scores and states are fp32 and enter the output's products as sums of two bf16 values (16 bits, where the output
+// keeps 8); decay^(C - 1 - j) v_j enters the state's as three (24 bits), since a state lives on. q, k and v are bf16.
+//
+// Few heads do not fill the device, so a long sequence is cut into segments: a first launch adds up each one's own state
+// from k and v, a second runs over the segments' states, and in a third each segment starts from its own.
 #include "common.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 namespace bh {
@@ -21,7 +37,11 @@ struct LinearArgs {
     float* state_out;
     int64_t ld_q, ld_k, ld_v, ld_o;
     int B, H, KH, group, N, D, E;
-    int slices;   // of the value columns
+    int slices;      // of the value columns (token after token)
+    float* states;   // [batch * kv_heads][segments][D][E]: the state before each segment
+    int segments, length;   // tokens of a segment, a multiple of kChunk
+    int first_state;        // the first segment's: 0 zeros, 1 state_in, 2 states
+    int heads_each;         // query heads that a workgroup takes one after the other: 1, or the group
     float scale;
 };
 
@@ -105,16 +125,423 @@ __global__ void __launch_bounds__(kThreads) k_linear_tokens(LinearArgs a) {
             if (d0 + 32 * p < a.D) *reinterpret_cast<f32x4_t*>(a.state_out + state + static_cast<int64_t>(d0 + 32 * p) * a.E) = s[p];
 }
 
+// ---- chunks ------------------------------------------------------------------------------------------
+
+constexpr int kChunk = 32;
+constexpr int kStages = 3;
+constexpr float kLog2e = 1.4426950408889634f;
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef short s16x8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
+// 16-byte chunks of a row of an LDS image, a power of two; chunk n of row r stands at place n ^ turn(r). 16 rows of one
+// chunk (a fragment) and four rows of two (half a transposing read takes eight rows) then lie in different banks.
+constexpr int places(int steps) { return steps == 1 ? 4 : steps == 2 ? 8 : 16; }
+template <int P>
+__device__ __forceinline__ int turn(int row) {
+    constexpr int bits = P == 4 ? 2 : P == 8 ? 3 : 4;
+    const int q = (row & 15) / (16 / P);
+    return ((q << 1) | (q >> (bits - 1))) & (P - 1);
+}
+
+// Byte offset that lane `lane` of load n of an image brings from memory: rows from last_row on repeat it, chunks from
+// `chunks` on the last one.
+template <int P>
+__device__ __forceinline__ uint32_t source(int n, int lane, int chunks, int last_row, uint32_t ld_bytes) {
+    const int id = n * 64 + lane, row = id / P, chunk = (id % P) ^ turn<P>(row);
+    return static_cast<uint32_t>(min(row, last_row)) * ld_bytes + static_cast<uint32_t>(min(chunk, chunks - 1)) * 16;
+}
+
+__device__ __forceinline__ s16x4_t read_transposed(const char* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(lds_address(p)));
+}
+__device__ __forceinline__ bf16x8_t pair(u32x2_t x, u32x2_t y) {
+    return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3));
+}
+__device__ __forceinline__ f32x4_t product(bf16x8_t a, bf16x8_t b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+// The bf16 nearest to each value, and what is left of the values.
+__device__ __forceinline__ u32x2_t take_bf16(f32x4_t& v) {
+    const u32x2_t h = {f2bf2(v[0], v[1]), f2bf2(v[2], v[3])};
+    v[0] -= __uint_as_float(h[0] << 16);
+    v[1] -= __uint_as_float(h[0] & 0xffff0000u);
+    v[2] -= __uint_as_float(h[1] << 16);
+    v[3] -= __uint_as_float(h[1] & 0xffff0000u);
+    return h;
+}
+
+// STEPS: of 32 columns of q and k; TILES: of 16 value columns a wave. Without OUT only the state is formed.
+template <int STEPS, int TILES, bool OUT>
+__global__ void __launch_bounds__(kThreads, 2) k_linear_chunks(LinearArgs a) {
+    constexpr int P = places(STEPS), PV = places(2 * TILES), DT = 2 * STEPS;
+    constexpr int kLoadsQ = OUT ? P / 2 : 0, kLoadsK = P / 2, kLoads = kLoadsQ + kLoadsK + PV / 2;   // of 1 KiB
+    constexpr int kItems = (kLoads + 3) / 4;                                                         // a wave's
+    constexpr int kStage = kLoads * 1024;
+    __shared__ __attribute__((aligned(1024))) char smem[kStages * kStage];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int per = OUT ? a.group / a.heads_each : 1, segments = OUT ? a.segments : a.segments - 1;
+    const int64_t T = static_cast<int64_t>(a.B) * a.KH * segments * per, number = group_index();
+    if (number >= T) return;
+    int64_t id = number;
+    if ((T & 7) == 0) id = (id & 7) * (T >> 3) + (id >> 3);   // heads of a group, which share keys, on one XCD
+    const int at = static_cast<int>(id % per), segment = static_cast<int>(id / per % segments);
+    const int64_t bk = id / per / segments;
+    const int kh = static_cast<int>(bk % a.KH), first = segment * a.length;
+    const int64_t b = bk / a.KH;
+    const int n = a.lens ? min(max(a.lens[b], 0), a.N) : a.N, last_segment = n > 0 ? (n - 1) / a.length : 0;
+    if (!OUT && segment >= last_segment) return;
+    const int count = min(max(n - first, 0), a.length), chunks = (count + kChunk - 1) / kChunk;
+    const float log_decay = log_decay_of(a, kh), rate = log_decay * kLog2e;
+    const Fade fade(kChunk * log_decay);
+    const int column = wave * TILES * 16;   // the wave's first value column
+    const bool active = column < a.E;
+
+    const uint32_t ldq = static_cast<uint32_t>(a.ld_q) * 2, ldk = static_cast<uint32_t>(a.ld_k) * 2, ldv = static_cast<uint32_t>(a.ld_v) * 2;
+    const int dc = a.D / 8, ec = a.E / 8;
+    auto offset = [&](int m, int last_row) {
+        return m < kLoadsQ             ? source<P>(m, lane, dc, last_row, ldq)
+               : m < kLoadsQ + kLoadsK ? source<P>(m - kLoadsQ, lane, dc, last_row, ldk)
+                                       : source<PV>(m - kLoadsQ - kLoadsK, lane, ec, last_row, ldv);
+    };
+    uint32_t off[kItems];   // (a wave beyond the last load repeats it)
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) off[i] = offset(min(i * 4 + wave, kLoads - 1), kChunk - 1);
+    const int64_t row0 = b * a.N + first;
+    const bf16_t* k0 = a.k + row0 * a.ld_k + static_cast<int64_t>(kh) * a.D;
+    const bf16_t* v0 = a.v + row0 * a.ld_v + static_cast<int64_t>(kh) * a.E;
+
+    // where this lane's fragments start in an image: rows c (of q and k) and 4 g + c / 4 (transposed)
+    const int frag = c * P * 16 + (((g >> 1) ^ turn<P>(c)) * 16) + (g & 1) * 8;
+    const int trow = 4 * g + (c >> 2);
+    const int kt = trow * P * 16 + ((((c & 3) >> 1) ^ turn<P>(trow)) * 16) + (c & 1) * 8;
+    const int vt = trow * PV * 16 + ((((c & 3) >> 1) ^ turn<PV>(trow)) * 16) + (c & 1) * 8;
+
+    // powers of the decay: token j of the fragment's order before the chunk's end, and (times scale) query c of a tile
+    // against the keys of its own tile, of the one before, and the state
+    float to_end[8], own[4], before[4], since[2];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) to_end[e] = exp2f(rate * (kChunk - 1 - ((e & 4) * 4 + 4 * g + (e & 3))));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int gap = c - 4 * g - r;
+        own[r] = gap >= 0 ? exp2f(rate * gap) * a.scale : 0.f;
+        before[r] = exp2f(rate * (16 + gap)) * a.scale;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) since[u] = exp2f(rate * (16 * u + c + 1)) * a.scale;
+
+    for (int turn_of = 0; turn_of < (OUT ? a.heads_each : 1); ++turn_of) {
+        const int member = at + turn_of, head = kh * a.group + member;
+        const bf16_t* q0 = OUT ? a.q + row0 * a.ld_q + static_cast<int64_t>(head) * a.D : nullptr;
+        auto load = [&](int j) {
+            const int rows = count - j * kChunk;
+            const bf16_t *q = q0 + static_cast<int64_t>(j) * kChunk * a.ld_q, *k = k0 + static_cast<int64_t>(j) * kChunk * a.ld_k;
+            const bf16_t* v = v0 + static_cast<int64_t>(j) * kChunk * a.ld_v;
+            const char* to = smem + j % kStages * kStage;
+            auto from = [&](int m) { return m < kLoadsQ ? q : m < kLoadsQ + kLoadsK ? k : v; };
+            if (rows >= kChunk) {
+#pragma unroll
+                for (int i = 0; i < kItems; ++i) {
+                    const int m = min(i * 4 + wave, kLoads - 1);
+                    dma16_at(from(m), off[i], to + m * 1024);
+                }
+                return;
+            }
+#pragma unroll 1
+            for (int i = 0; i < kItems; ++i) {
+                const int m = min(i * 4 + wave, kLoads - 1);
+                dma16_at(from(m), offset(m, rows - 1), to + m * 1024);
+            }
+        };
+        if (chunks > 0) load(0);
+        if (chunks > 1) load(1);
+
+        // s[t][x][r]: row 16 t + 4 g + r, column 16 x + c of the wave's
+        f32x4_t s[DT][TILES];
+        const float* start = nullptr;
+        if (OUT) {
+            const int64_t size = static_cast<int64_t>(a.D) * a.E;
+            if (segment > 0 || a.first_state == 2) start = a.states + (bk * a.segments + segment) * size;
+            else if (a.first_state == 1) start = a.state_in + bk * size;
+        }
+        int from = lane;   // opaque, as below
+        asm volatile("" : "+v"(from));
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int x = 0; x < TILES; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int d = t * 16 + (from >> 4) * 4 + r, e = column + x * 16 + (from & 15);
+                    s[t][x][r] = start && d < a.D && e < a.E ? start[d * a.E + e] : 0.f;
+                }
+
+        u32x2_t done[TILES][2];   // the last chunk's outputs: they leave behind the next one's barrier
+        auto store = [&](int j, int rows) {
+#pragma unroll
+            for (int x = 0; x < TILES; ++x) {
+                const int e = column + x * 16 + g * 4;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int i = u * 16 + c;
+                    if (e < a.E && i < rows)
+                        *reinterpret_cast<u32x2_t*>(a.out + (row0 + j * kChunk + i) * a.ld_o + static_cast<int64_t>(head) * a.E + e) = done[x][u];
+                }
+            }
+        };
+        for (int j = 0; j < chunks; ++j) {
+            // this wave's loads of chunk j have landed, those of chunk j + 1 may be on their way; behind the barrier
+            // everyone's have, and chunk j - 1 has been read
+            asm volatile("" ::: "memory");
+            if (j + 1 < chunks) s_waitcnt<kItems, 0>();
+            else s_waitcnt<0, 0>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (OUT && j > 0) store(j - 1, kChunk);
+            if (j + 2 < chunks) load(j + 2);
+            if (!active) continue;
+            const int rows = min(count - j * kChunk, kChunk);
+            const char* image = smem + j % kStages * kStage;
+            const char *qi = image, *ki = image + kLoadsQ * 1024, *vi = ki + kLoadsK * 1024;
+
+            f32x4_t o[TILES][2];
+            bf16x8_t v[TILES];
+#pragma unroll
+            for (int x = 0; x < TILES; ++x) {
+                const char* p = vi + (vt ^ ((column / 8 + x * 2) * 16));
+                v[x] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(read_transposed(p), read_transposed(p + 16 * PV * 16), 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+            if (OUT) {
+                bf16x8_t qf[2][STEPS];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k) {
+                        u32x2_t h[2];
+#pragma unroll
+                        for (int z = 0; z < 2; ++z) {
+                            h[z] = *reinterpret_cast<const u32x2_t*>(qi + u * 16 * P * 16 + (frag ^ ((k * 4 + z * 2) * 16)));
+                            if (k == STEPS - 1 && k * 4 + z * 2 + (g >> 1) >= dc) h[z] = u32x2_t{0, 0};   // past head_dim
+                        }
+                        qf[u][k] = pair(h[0], h[1]);
+                    }
+                // scores of key tile y against query tile u >= y
+                f32x4_t score[3] = {};   // (0, 0), (0, 1), (1, 1)
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k) {
+                        u32x2_t h[2];
+#pragma unroll
+                        for (int z = 0; z < 2; ++z) h[z] = *reinterpret_cast<const u32x2_t*>(ki + y * 16 * P * 16 + (frag ^ ((k * 4 + z * 2) * 16)));
+                        const bf16x8_t kf = pair(h[0], h[1]);
+                        if (y == 0) score[0] = product(kf, qf[0][k], score[0]);
+                        score[1 + y] = product(kf, qf[1][k], score[1 + y]);
+                    }
+                // the state's part
+#pragma unroll
+                for (int x = 0; x < TILES; ++x) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) o[x][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k) {
+                        f32x4_t lo = s[2 * k][x], hi = s[2 * k + 1][x];
+                        const u32x2_t l1 = take_bf16(lo), h1 = take_bf16(hi);
+                        const bf16x8_t one = pair(l1, h1);
+                        const bf16x8_t two = pair(u32x2_t{f2bf2(lo[0], lo[1]), f2bf2(lo[2], lo[3])}, u32x2_t{f2bf2(hi[0], hi[1]), f2bf2(hi[2], hi[3])});
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            o[x][u] = product(one, qf[u][k], o[x][u]);
+                            o[x][u] = product(two, qf[u][k], o[x][u]);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[x][u][r] *= since[u];
+                }
+                // the chunk's own
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    score[0][r] *= own[r];
+                    score[1][r] *= before[r];
+                    score[2][r] *= own[r];
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    f32x4_t lo = score[u], hi = u == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : score[2];
+                    const u32x2_t l1 = take_bf16(lo), h1 = take_bf16(hi);
+                    const bf16x8_t one = pair(l1, h1);
+                    const bf16x8_t two = pair(u32x2_t{f2bf2(lo[0], lo[1]), f2bf2(lo[2], lo[3])}, u32x2_t{f2bf2(hi[0], hi[1]), f2bf2(hi[2], hi[3])});
+#pragma unroll
+                    for (int x = 0; x < TILES; ++x) {
+                        o[x][u] = product(v[x], one, o[x][u]);
+                        o[x][u] = product(v[x], two, o[x][u]);
+                        done[x][u] = u32x2_t{f2bf2(o[x][u][0], o[x][u][1]), f2bf2(o[x][u][2], o[x][u][3])};
+                    }
+                }
+            }
+            // the state behind the chunk
+            float weight[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) weight[e] = to_end[e];
+            Fade by = fade;
+            if (rows < kChunk) {
+                by = Fade(rows * log_decay);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int left = rows - 1 - ((e & 4) * 4 + 4 * g + (e & 3));
+                    weight[e] = left >= 0 ? exp2f(rate * left) : 0.f;
+                }
+            }
+            bf16x8_t w[TILES][3];
+#pragma unroll
+            for (int x = 0; x < TILES; ++x) {
+                const u32x4_t raw = __builtin_bit_cast(u32x4_t, v[x]);
+                f32x4_t lo, hi;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    lo[2 * e] = __uint_as_float(raw[e] << 16) * weight[2 * e];
+                    lo[2 * e + 1] = __uint_as_float(raw[e] & 0xffff0000u) * weight[2 * e + 1];
+                    hi[2 * e] = __uint_as_float(raw[2 + e] << 16) * weight[4 + 2 * e];
+                    hi[2 * e + 1] = __uint_as_float(raw[2 + e] & 0xffff0000u) * weight[4 + 2 * e + 1];
+                }
+#pragma unroll
+                for (int z = 0; z < 3; ++z) {
+                    const u32x2_t l = take_bf16(lo), h = take_bf16(hi);
+                    w[x][z] = pair(l, h);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                const char* p = ki + (kt ^ (t * 2 * 16));
+                const bf16x8_t kf = __builtin_bit_cast(
+                    bf16x8_t, __builtin_shufflevector(read_transposed(p), read_transposed(p + 16 * P * 16), 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int x = 0; x < TILES; ++x) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[t][x][r] = by(s[t][x][r]);
+#pragma unroll
+                    for (int z = 2; z >= 0; --z) s[t][x] = product(kf, w[x][z], s[t][x]);
+                }
+            }
+        }
+        if (OUT && chunks > 0 && active) store(chunks - 1, count - (chunks - 1) * kChunk);
+        float* end = nullptr;
+        if (!OUT) end = a.states + (bk * a.segments + segment + 1) * a.D * a.E;
+        else if (a.state_out && segment == last_segment && member == a.group - 1) end = a.state_out + bk * a.D * a.E;
+        if (end) {
+            int here = lane;   // computed anew: the offsets of the first state's values would stay in registers through the loop
+            asm volatile("" : "+v"(here));
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int x = 0; x < TILES; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int d = t * 16 + (here >> 4) * 4 + r, e = column + x * 16 + (here & 15);
+                        if (d < a.D && e < a.E) end[d * a.E + e] = s[t][x][r];
+                    }
+        }
+        if (OUT) {   // the outputs behind the sequence
+            const int behind = max(n - first, 0), rows = min(a.N - first, a.length);
+            const int pieces = a.E / 4;
+            for (int i = threadIdx.x; i < (rows - behind) * pieces; i += kThreads) {
+                const int64_t row = row0 + behind + i / pieces;
+                *reinterpret_cast<uint2*>(a.out + row * a.ld_o + static_cast<int64_t>(head) * a.E + i % pieces * 4) = make_uint2(0, 0);
+            }
+            if (turn_of + 1 < a.heads_each) {   // the next head's loads reuse the stages
+                asm volatile("" ::: "memory");
+                s_waitcnt<0, 0>();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+            }
+        }
+    }
+}
+
+// The segments' own states, each before the next one's place, become the states before them; the first is state_in or zeros.
+__global__ void __launch_bounds__(kThreads) k_linear_carry(LinearArgs a) {
+    const int64_t size = static_cast<int64_t>(a.D) * a.E / 4, i = group_index() * kThreads + threadIdx.x;
+    const int64_t bk = i / size;
+    if (bk >= static_cast<int64_t>(a.B) * a.KH) return;
+    const int64_t b = bk / a.KH;
+    const int n = a.lens ? min(max(a.lens[b], 0), a.N) : a.N, last = n > 0 ? (n - 1) / a.length : 0;
+    const Fade fade(static_cast<float>(a.length) * log_decay_of(a, static_cast<int>(bk % a.KH)));
+    f32x4_t s = a.state_in ? reinterpret_cast<const f32x4_t*>(a.state_in)[i] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+    f32x4_t* at = reinterpret_cast<f32x4_t*>(a.states) + bk * a.segments * size + (i - bk * size);
+    *at = s;
+    for (int m = 1; m <= last; ++m) {
+        at += size;
+        const f32x4_t own = *at;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = fade(s[r]) + own[r];
+        *at = s;
+    }
+}
+
+int device_cus() {
+    static std::atomic<int> cus[64] = {};
+    int dev = 0;
+    hip_check(hipGetDevice(&dev), "hipGetDevice");
+    require(dev >= 0 && dev < 64, "attention_linear: device index out of range");
+    int n = cus[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        hip_check(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev), "hipDeviceGetAttribute");
+        require(n > 0, "attention_linear: device reports no compute units");
+        cus[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+struct Plan {
+    bool tokens;    // k_linear_tokens
+    int segments, length;
+};
+Plan plan(const LinearShape& sh, bool may_split, int64_t cus) {
+    if (sh.seq_len <= 16) return Plan{true, 1, static_cast<int>(sh.seq_len)};
+    const int64_t chunks = (sh.seq_len + kChunk - 1) / kChunk, heads = sh.batch * sh.heads;
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(chunks / 4, (2 * cus + heads - 1) / heads));
+    const int64_t each = may_split ? (chunks + most - 1) / most : chunks;
+    return Plan{false, static_cast<int>((chunks + each - 1) / each), static_cast<int>(each * kChunk)};
+}
+
+template <int STEPS, int TILES, bool OUT>
+void launch(const LinearArgs& a, int64_t groups, hipStream_t s) {
+    k_linear_chunks<STEPS, TILES, OUT><<<grid_of(groups, kThreads), kThreads, 0, s>>>(a);
+    launch_check("attention_linear");
+}
+template <bool OUT>
+void by_width(const LinearArgs& a, int64_t groups, hipStream_t s) {
+    const bool wide = a.E > 64;
+    switch ((a.D + 31) / 32) {
+        case 1: return wide ? launch<1, 2, OUT>(a, groups, s) : launch<1, 1, OUT>(a, groups, s);
+        case 2: return wide ? launch<2, 2, OUT>(a, groups, s) : launch<2, 1, OUT>(a, groups, s);
+        case 3: return wide ? launch<3, 2, OUT>(a, groups, s) : launch<3, 1, OUT>(a, groups, s);
+        default: return wide ? launch<4, 2, OUT>(a, groups, s) : launch<4, 1, OUT>(a, groups, s);
+    }
+}
+
 }  // namespace
 
-int64_t attention_linear_workspace_floats(const LinearShape&) { return 0; }
+int64_t attention_linear_workspace_floats(const LinearShape& sh) {
+    const Plan how = plan(sh, true, device_cus());
+    const int64_t states = sh.batch * sh.kv_heads * sh.head_dim * sh.value_dim;
+    // one state each where a group's heads would still read what one of them writes
+    return how.segments > 1 ? how.segments * states : !how.tokens && sh.heads > sh.kv_heads ? states : 0;
+}
 
-bh_attention_linear_plan attention_linear_plan(const LinearShape& sh, bool, int) {
-    return bh_attention_linear_plan{1, 1, sh.batch * sh.kv_heads * ((sh.value_dim + 31) / 32)};
+bh_attention_linear_plan attention_linear_plan(const LinearShape& sh, bool may_split, int cus) {
+    const Plan how = plan(sh, may_split, cus > 0 ? cus : device_cus());
+    if (how.tokens) return bh_attention_linear_plan{1, 1, sh.batch * sh.kv_heads * ((sh.value_dim + 31) / 32)};
+    return bh_attention_linear_plan{kChunk, how.segments, sh.batch * sh.heads * how.segments};
 }
 
 void launch_attention_linear(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16_t* out, const LinearShape& sh,
-                             const float* log_decay, const int32_t* lens, const float* state_in, float* state_out, float*,
+                             const float* log_decay, const int32_t* lens, const float* state_in, float* state_out, float* ws,
                              hipStream_t s) {
     LinearArgs a;
     a.q = q; a.k = k; a.v = v; a.out = out;
@@ -126,10 +553,30 @@ void launch_attention_linear(const bf16_t* q, const bf16_t* k, const bf16_t* v, 
     a.N = static_cast<int>(sh.seq_len); a.D = static_cast<int>(sh.head_dim); a.E = static_cast<int>(sh.value_dim);
     a.slices = (a.E + 31) / 32;
     a.scale = sh.scale;
+    const Plan how = plan(sh, ws != nullptr, device_cus());
+    a.states = ws;
+    a.segments = how.segments;
+    a.length = how.length;
     ProfileScope ps(K_ATTN_SELF, s, 2.0 * sh.batch * sh.seq_len * (sh.heads + sh.kv_heads) * sh.head_dim * sh.value_dim);
-    const int64_t groups = sh.batch * sh.kv_heads * a.slices;
-    k_linear_tokens<<<grid_of(groups, kThreads), kThreads, 0, s>>>(a);
-    launch_check("attention_linear");
+    const int64_t rows = sh.batch * sh.kv_heads;
+    if (how.tokens) {
+        k_linear_tokens<<<grid_of(rows * a.slices, kThreads), kThreads, 0, s>>>(a);
+        launch_check("attention_linear");
+        return;
+    }
+    // a group's workgroups read the first state while one of them may end and write it in place
+    const bool in_place = state_in && state_in == state_out && a.group > 1;
+    const bool copied = how.segments > 1 || (in_place && ws);
+    a.first_state = copied ? 2 : state_in ? 1 : 0;
+    a.heads_each = in_place && !copied ? a.group : 1;
+    const int64_t groups = rows * how.segments * (a.group / a.heads_each);
+    require(groups < (int64_t{1} << 40), "attention_linear: too many heads");
+    if (how.segments > 1) by_width<false>(a, rows * (how.segments - 1), s);
+    if (copied) {
+        k_linear_carry<<<grid_of((rows * a.D * a.E / 4 + kThreads - 1) / kThreads, kThreads), kThreads, 0, s>>>(a);
+        launch_check("attention_linear");
+    }
+    by_width<true>(a, groups, s);
 }
 
 }  // namespace bh

@@ -329,6 +329,27 @@ def test_offsets_beyond_32_bits(hip):
     compare(out, want, tol)
 
 
+def test_stays_inside_its_workspace_and_refuses_a_small_one(hip):
+    import torch
+    q, k, v = inputs(1, 4, 2, 3000, 64, 64, 1)
+    rate, out = decays(2), torch.zeros(1, 3000, 4, 64, dtype=torch.bfloat16, device="cuda")
+    new = torch.zeros(1, 2, 64, 64, device="cuda")
+    _, need = workspace(q, k, v)
+    assert need > 0
+    ws = torch.full((need + 4096,), 0x5a, dtype=torch.uint8, device="cuda")
+    with pytest.raises(bh.BurnisherError, match="this call needs"):
+        call(q, k, v, out, rate, None, None, new, 0.0, ws, need - 1)
+    with pytest.raises(bh.BurnisherError, match="16-byte"):
+        call(q, k, v, out, rate, None, None, new, 0.0, ws[4:], need)
+    torch.cuda.synchronize()
+    assert not out.any() and not new.any() and (ws == 0x5a).all(), "a refused call wrote"
+    call(q, k, v, out, rate, None, None, new, 0.0, ws, need)
+    torch.cuda.synchronize()
+    assert (ws[need:] == 0x5a).all(), "written past the workspace"
+    again, state = run(q, k, v, rate)
+    assert torch.equal(out, again) and torch.equal(new, state)
+
+
 @pytest.mark.parametrize("n", [1, 50, 2500])
 def test_in_a_graph_and_on_two_streams(hip, n):
     import torch
