@@ -7,8 +7,9 @@
 // four matrix products, all on v_mfma_f32_16x16x32_bf16. A workgroup's waves share a chunk of q, k and v in LDS and
 // each keep 16 or 32 columns of the state in accumulators for all chunks; every wave computes the chunk's
 // scores anew (12 of its 100 matrix instructions at 128 x 128). Products are formed transposed, S and out^T from V^T, so
-// that two accumulator tiles of 16 rows, of scores or state, are one operand of the next product, in an order of its
-// 32 columns (4 g + r, then 16 + 4 g + r for lane group g) that the other operand's loads follow.
+// that two accumulator tiles of 16 rows, of scores or state, are one operand of the next product. The order of its
+// 32 columns is followed by the other operand: tokens 4 g + r, then 16 + 4 g + r for lane group g (v); the state's
+// rows are dealt to its tiles so that theirs is 8 g .. 8 g + 7, 16 bytes of q.
 //
 // Scores and states are fp32 and enter the output's products as sums of two bf16 values (16 bits, where the output
 // keeps 8); decay^(C - 1 - j) v_j enters the state's as three (24 bits), since a state lives on. q, k and v are bf16.
@@ -38,8 +39,10 @@ struct LinearArgs {
     int64_t ld_q, ld_k, ld_v, ld_o;
     int B, H, KH, group, N, D, E;
     int slices;      // of the value columns (token after token)
-    float* states;   // [batch * kv_heads][segments][D][E]: the state before each segment
-    int segments, length;   // tokens of a segment, a multiple of kChunk
+    // [batch * kv_heads][1 + (segments - 1) * pieces][D][E]: place m + 1 first takes the own state of piece m, and then
+    // place n * pieces the state before segment n
+    float* states;
+    int segments, pieces, length;   // of a sequence, of a segment, tokens of a piece (a multiple of kChunk)
     int first_state;        // the first segment's: 0 zeros, 1 state_in, 2 states
     int heads_each;         // query heads that a workgroup takes one after the other: 1, or the group
     float scale;
@@ -136,21 +139,23 @@ typedef short s16x8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
-// 16-byte chunks of a row of an LDS image, a power of two; chunk n of row r stands at place n ^ turn(r). 16 rows of one
-// chunk (a fragment) and four rows of two (half a transposing read takes eight rows) then lie in different banks.
+// 16-byte chunks of a row of an LDS image, a power of two; chunk n of row r stands at place n ^ turn(r), r / (16 / P) with
+// its bits rotated by BY. Rows c of one chunk (a fragment: 16 bytes a lane, eight lanes at a time) then lie in different
+// banks. Of the transposing reads, eight rows at a time, those of two whole chunks (v: BY 1) do too; those of half of four
+// chunks each (k: BY 2), whose order lets a fragment be one read, meet in pairs.
 constexpr int places(int steps) { return steps == 1 ? 4 : steps == 2 ? 8 : 16; }
-template <int P>
+template <int P, int BY>
 __device__ __forceinline__ int turn(int row) {
-    constexpr int bits = P == 4 ? 2 : P == 8 ? 3 : 4;
+    constexpr int bits = P == 4 ? 2 : P == 8 ? 3 : 4, by = BY % bits;
     const int q = (row & 15) / (16 / P);
-    return ((q << 1) | (q >> (bits - 1))) & (P - 1);
+    return ((q << by) | (q >> (bits - by))) & (P - 1);
 }
 
 // Byte offset that lane `lane` of load n of an image brings from memory: rows from last_row on repeat it, chunks from
 // `chunks` on the last one.
-template <int P>
+template <int P, int BY>
 __device__ __forceinline__ uint32_t source(int n, int lane, int chunks, int last_row, uint32_t ld_bytes) {
-    const int id = n * 64 + lane, row = id / P, chunk = (id % P) ^ turn<P>(row);
+    const int id = n * 64 + lane, row = id / P, chunk = (id % P) ^ turn<P, BY>(row);
     return static_cast<uint32_t>(min(row, last_row)) * ld_bytes + static_cast<uint32_t>(min(chunk, chunks - 1)) * 16;
 }
 
@@ -165,7 +170,8 @@ __device__ __forceinline__ f32x4_t product(bf16x8_t a, bf16x8_t b, f32x4_t c) {
 }
 // The bf16 nearest to each value, and what is left of the values.
 __device__ __forceinline__ u32x2_t take_bf16(f32x4_t& v) {
-    const u32x2_t h = {f2bf2(v[0], v[1]), f2bf2(v[2], v[3])};
+    u32x2_t h = {f2bf2(v[0], v[1]), f2bf2(v[2], v[3])};
+    asm("" : "+v"(h));   // one conversion: the compiler would convert each value again to get it alone
     v[0] -= __uint_as_float(h[0] << 16);
     v[1] -= __uint_as_float(h[0] & 0xffff0000u);
     v[2] -= __uint_as_float(h[1] << 16);
@@ -173,51 +179,59 @@ __device__ __forceinline__ u32x2_t take_bf16(f32x4_t& v) {
     return h;
 }
 
-// STEPS: of 32 columns of q and k; TILES: of 16 value columns a wave. Without OUT only the state is formed.
-template <int STEPS, int TILES, bool OUT>
-__global__ void __launch_bounds__(kThreads, 2) k_linear_chunks(LinearArgs a) {
-    constexpr int P = places(STEPS), PV = places(2 * TILES), DT = 2 * STEPS;
+// STEPS: of 32 columns of q and k; TILES: of 16 value columns a wave. With OUT a workgroup walks a segment for one query
+// head from the state before it. Without, it adds up a piece's own state from k and v, from its end back, so that
+// weights only fall and the walk ends where they are zero, and what it read last is what the next launch reads first.
+template <int STEPS, int TILES, int WAVES, bool OUT>
+__global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
+    constexpr int P = places(STEPS), PV = places(WAVES * TILES / 2), DT = 2 * STEPS;
     constexpr int kLoadsQ = OUT ? P / 2 : 0, kLoadsK = P / 2, kLoads = kLoadsQ + kLoadsK + PV / 2;   // of 1 KiB
-    constexpr int kItems = (kLoads + 3) / 4;                                                         // a wave's
+    constexpr int kItems = (kLoads + WAVES - 1) / WAVES;                                             // a wave's
     constexpr int kStage = kLoads * 1024;
     __shared__ __attribute__((aligned(1024))) char smem[kStages * kStage];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-    const int per = OUT ? a.group / a.heads_each : 1, segments = OUT ? a.segments : a.segments - 1;
-    const int64_t T = static_cast<int64_t>(a.B) * a.KH * segments * per, number = group_index();
+    const int per = OUT ? a.group / a.heads_each : 1, segments = OUT ? a.segments : (a.segments - 1) * a.pieces;
+    const int64_t number = group_index();
+    const int T = a.B * a.KH * segments * per;
     if (number >= T) return;
-    int64_t id = number;
+    int id = static_cast<int>(number);
     if ((T & 7) == 0) id = (id & 7) * (T >> 3) + (id >> 3);   // heads of a group, which share keys, on one XCD
-    const int at = static_cast<int>(id % per), segment = static_cast<int>(id / per % segments);
+    const int at = id % per, segment = id / per % segments;
     const int64_t bk = id / per / segments;
-    const int kh = static_cast<int>(bk % a.KH), first = segment * a.length;
-    const int64_t b = bk / a.KH;
-    const int n = a.lens ? min(max(a.lens[b], 0), a.N) : a.N, last_segment = n > 0 ? (n - 1) / a.length : 0;
-    if (!OUT && segment >= last_segment) return;
-    const int count = min(max(n - first, 0), a.length), chunks = (count + kChunk - 1) / kChunk;
+    const int length = OUT ? a.length * a.pieces : a.length, first = segment * length;
+    const int kh = static_cast<int>(bk) % a.KH;
+    const int64_t b = static_cast<int>(bk) / a.KH;
+    const int n = a.lens ? min(max(a.lens[b], 0), a.N) : a.N, last_segment = n > 0 ? (n - 1) / (a.length * a.pieces) : 0;
+    if (!OUT && segment >= last_segment * a.pieces) return;
     const float log_decay = log_decay_of(a, kh), rate = log_decay * kLog2e;
-    const Fade fade(kChunk * log_decay);
+    const int count = min(max(n - first, 0), length);
+    // a weight below 2^-150 is zero
+    const int chunks = OUT ? (count + kChunk - 1) / kChunk : min(length / kChunk, static_cast<int>(1.f + 150.f / fmaxf(-rate * kChunk, 1e-6f)));
     const int column = wave * TILES * 16;   // the wave's first value column
     const bool active = column < a.E;
+    auto column_of = [&](int x, int i) { return column + (TILES == 2 ? (i >> 2) * 8 + x * 4 + (i & 3) : i); };   // row or column i of tile x
 
     const uint32_t ldq = static_cast<uint32_t>(a.ld_q) * 2, ldk = static_cast<uint32_t>(a.ld_k) * 2, ldv = static_cast<uint32_t>(a.ld_v) * 2;
     const int dc = a.D / 8, ec = a.E / 8;
     auto offset = [&](int m, int last_row) {
-        return m < kLoadsQ             ? source<P>(m, lane, dc, last_row, ldq)
-               : m < kLoadsQ + kLoadsK ? source<P>(m - kLoadsQ, lane, dc, last_row, ldk)
-                                       : source<PV>(m - kLoadsQ - kLoadsK, lane, ec, last_row, ldv);
+        return m < kLoadsQ             ? source<P, 2>(m, lane, dc, last_row, ldq)
+               : m < kLoadsQ + kLoadsK ? source<P, 2>(m - kLoadsQ, lane, dc, last_row, ldk)
+                                       : source<PV, TILES>(m - kLoadsQ - kLoadsK, lane, ec, last_row, ldv);
     };
     uint32_t off[kItems];   // (a wave beyond the last load repeats it)
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) off[i] = offset(min(i * 4 + wave, kLoads - 1), kChunk - 1);
+    for (int i = 0; i < kItems; ++i) off[i] = offset(min(i * WAVES + wave, kLoads - 1), kChunk - 1);
     const int64_t row0 = b * a.N + first;
     const bf16_t* k0 = a.k + row0 * a.ld_k + static_cast<int64_t>(kh) * a.D;
     const bf16_t* v0 = a.v + row0 * a.ld_v + static_cast<int64_t>(kh) * a.E;
 
-    // where this lane's fragments start in an image: rows c (of q and k) and 4 g + c / 4 (transposed)
-    const int frag = c * P * 16 + (((g >> 1) ^ turn<P>(c)) * 16) + (g & 1) * 8;
+    // where this lane's fragments start in an image: chunk g of row c (of q and k), and of row 4 g + c / 4, transposed, half
+    // of chunk c % 4 (k, and v in two tiles, whose columns are dealt as the state's rows) or a quarter of chunks 0 and 1
     const int trow = 4 * g + (c >> 2);
-    const int kt = trow * P * 16 + ((((c & 3) >> 1) ^ turn<P>(trow)) * 16) + (c & 1) * 8;
-    const int vt = trow * PV * 16 + ((((c & 3) >> 1) ^ turn<PV>(trow)) * 16) + (c & 1) * 8;
+    const int frag = c * P * 16 + (g ^ turn<P, 2>(c)) * 16;
+    const int kt = trow * P * 16 + ((c & 3) ^ turn<P, 2>(trow)) * 16;
+    const int vt = TILES == 2 ? trow * PV * 16 + ((c & 3) ^ turn<PV, 2>(trow)) * 16
+                              : trow * PV * 16 + (((c & 3) >> 1) ^ turn<PV, 1>(trow)) * 16 + (c & 1) * 8;
 
     // powers of the decay: token j of the fragment's order before the chunk's end, and (times scale) query c of a tile
     // against the keys of its own tile, of the one before, and the state
@@ -237,34 +251,34 @@ __global__ void __launch_bounds__(kThreads, 2) k_linear_chunks(LinearArgs a) {
         const int member = at + turn_of, head = kh * a.group + member;
         const bf16_t* q0 = OUT ? a.q + row0 * a.ld_q + static_cast<int64_t>(head) * a.D : nullptr;
         auto load = [&](int j) {
-            const int rows = count - j * kChunk;
-            const bf16_t *q = q0 + static_cast<int64_t>(j) * kChunk * a.ld_q, *k = k0 + static_cast<int64_t>(j) * kChunk * a.ld_k;
-            const bf16_t* v = v0 + static_cast<int64_t>(j) * kChunk * a.ld_v;
+            const int64_t t = OUT ? j * kChunk : length - (j + 1) * kChunk;
+            const int rows = OUT ? count - j * kChunk : kChunk;
+            const bf16_t *q = q0 + t * a.ld_q, *k = k0 + t * a.ld_k, *v = v0 + t * a.ld_v;
             const char* to = smem + j % kStages * kStage;
             auto from = [&](int m) { return m < kLoadsQ ? q : m < kLoadsQ + kLoadsK ? k : v; };
             if (rows >= kChunk) {
 #pragma unroll
                 for (int i = 0; i < kItems; ++i) {
-                    const int m = min(i * 4 + wave, kLoads - 1);
+                    const int m = min(i * WAVES + wave, kLoads - 1);
                     dma16_at(from(m), off[i], to + m * 1024);
                 }
                 return;
             }
 #pragma unroll 1
             for (int i = 0; i < kItems; ++i) {
-                const int m = min(i * 4 + wave, kLoads - 1);
+                const int m = min(i * WAVES + wave, kLoads - 1);
                 dma16_at(from(m), offset(m, rows - 1), to + m * 1024);
             }
         };
         if (chunks > 0) load(0);
         if (chunks > 1) load(1);
 
-        // s[t][x][r]: row 16 t + 4 g + r, column 16 x + c of the wave's
+        // s[t][x][r]: row 32 (t / 2) + 8 g + 4 (t % 2) + r, column column_of(x, c)
         f32x4_t s[DT][TILES];
         const float* start = nullptr;
         if (OUT) {
             const int64_t size = static_cast<int64_t>(a.D) * a.E;
-            if (segment > 0 || a.first_state == 2) start = a.states + (bk * a.segments + segment) * size;
+            if (segment > 0 || a.first_state == 2) start = a.states + (bk * (1 + (a.segments - 1) * a.pieces) + segment * a.pieces) * size;
             else if (a.first_state == 1) start = a.state_in + bk * size;
         }
         int from = lane;   // opaque, as below
@@ -275,21 +289,24 @@ __global__ void __launch_bounds__(kThreads, 2) k_linear_chunks(LinearArgs a) {
             for (int x = 0; x < TILES; ++x)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int d = t * 16 + (from >> 4) * 4 + r, e = column + x * 16 + (from & 15);
+                    const int d = t / 2 * 32 + (from >> 4) * 8 + t % 2 * 4 + r, e = column_of(x, from & 15);
                     s[t][x][r] = start && d < a.D && e < a.E ? start[d * a.E + e] : 0.f;
                 }
 
-        u32x2_t done[TILES][2];   // the last chunk's outputs: they leave behind the next one's barrier
+        // The state is `faded` times what the accumulators hold: its decay is put off, as a factor of what is added, until
+        // it comes to 2^-8 since `age` tokens. Applied in every chunk it took 128 of 650 vector instructions.
+        int age = 0;
+        float faded = 1.f;
+        typedef uint32_t out_t __attribute__((ext_vector_type(2 * TILES)));
+        out_t done[2];   // the last chunk's outputs, columns column_of(0, 4 g) on of query c: they leave behind the next barrier
         auto store = [&](int j, int rows) {
+            const int e = column_of(0, g * 4);
 #pragma unroll
-            for (int x = 0; x < TILES; ++x) {
-                const int e = column + x * 16 + g * 4;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int i = u * 16 + c;
-                    if (e < a.E && i < rows)
-                        *reinterpret_cast<u32x2_t*>(a.out + (row0 + j * kChunk + i) * a.ld_o + static_cast<int64_t>(head) * a.E + e) = done[x][u];
-                }
+            for (int u = 0; u < 2; ++u) {
+                const int i = u * 16 + c;
+                typedef out_t Any __attribute__((aligned(8)));
+                if (e < a.E && i < rows)
+                    *reinterpret_cast<Any*>(a.out + (row0 + j * kChunk + i) * a.ld_o + static_cast<int64_t>(head) * a.E + e) = done[u];
             }
         };
         for (int j = 0; j < chunks; ++j) {
@@ -301,67 +318,59 @@ __global__ void __launch_bounds__(kThreads, 2) k_linear_chunks(LinearArgs a) {
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
             if (OUT && j > 0) store(j - 1, kChunk);
-            if (j + 2 < chunks) load(j + 2);
-            if (!active) continue;
+            if (!active) {
+                if (j + 2 < chunks) load(j + 2);
+                continue;
+            }
             const int rows = min(count - j * kChunk, kChunk);
             const char* image = smem + j % kStages * kStage;
             const char *qi = image, *ki = image + kLoadsQ * 1024, *vi = ki + kLoadsK * 1024;
 
-            f32x4_t o[TILES][2];
+            auto read_values = [&](int x) {
+                const char* p = vi + (vt ^ (column / 8 * 16)) + x * 8;
+                return __builtin_bit_cast(
+                    bf16x8_t, __builtin_shufflevector(read_transposed(p), read_transposed(p + 16 * PV * 16), 0, 1, 2, 3, 4, 5, 6, 7));
+            };
             bf16x8_t v[TILES];
-#pragma unroll
-            for (int x = 0; x < TILES; ++x) {
-                const char* p = vi + (vt ^ ((column / 8 + x * 2) * 16));
-                v[x] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(read_transposed(p), read_transposed(p + 16 * PV * 16), 0, 1, 2, 3, 4, 5, 6, 7));
-            }
             if (OUT) {
-                bf16x8_t qf[2][STEPS];
+                // by 32 rows of the state: scores of key tile y against query tile u >= y, and the state's part of the outputs
+                const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+                __builtin_amdgcn_s_setprio(1);
+                f32x4_t o[TILES][2], score[3];   // (0, 0), (0, 1), (1, 1)
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int k = 0; k < STEPS; ++k) {
+                    bf16x8_t qf[2], kf[2];
 #pragma unroll
-                    for (int k = 0; k < STEPS; ++k) {
-                        u32x2_t h[2];
-#pragma unroll
-                        for (int z = 0; z < 2; ++z) {
-                            h[z] = *reinterpret_cast<const u32x2_t*>(qi + u * 16 * P * 16 + (frag ^ ((k * 4 + z * 2) * 16)));
-                            if (k == STEPS - 1 && k * 4 + z * 2 + (g >> 1) >= dc) h[z] = u32x2_t{0, 0};   // past head_dim
-                        }
-                        qf[u][k] = pair(h[0], h[1]);
+                    for (int u = 0; u < 2; ++u) {
+                        u32x4_t f = *reinterpret_cast<const u32x4_t*>(qi + u * 16 * P * 16 + (frag ^ (k * 64)));
+                        if (k == STEPS - 1 && k * 4 + g >= dc) f = u32x4_t{0, 0, 0, 0};   // past head_dim
+                        qf[u] = __builtin_bit_cast(bf16x8_t, f);
+                        kf[u] = *reinterpret_cast<const bf16x8_t*>(ki + u * 16 * P * 16 + (frag ^ (k * 64)));
                     }
-                // scores of key tile y against query tile u >= y
-                f32x4_t score[3] = {};   // (0, 0), (0, 1), (1, 1)
+                    score[0] = product(kf[0], qf[0], k == 0 ? zero : score[0]);
+                    score[1] = product(kf[0], qf[1], k == 0 ? zero : score[1]);
+                    score[2] = product(kf[1], qf[1], k == 0 ? zero : score[2]);
 #pragma unroll
-                for (int y = 0; y < 2; ++y)
-#pragma unroll
-                    for (int k = 0; k < STEPS; ++k) {
-                        u32x2_t h[2];
-#pragma unroll
-                        for (int z = 0; z < 2; ++z) h[z] = *reinterpret_cast<const u32x2_t*>(ki + y * 16 * P * 16 + (frag ^ ((k * 4 + z * 2) * 16)));
-                        const bf16x8_t kf = pair(h[0], h[1]);
-                        if (y == 0) score[0] = product(kf, qf[0][k], score[0]);
-                        score[1 + y] = product(kf, qf[1][k], score[1 + y]);
-                    }
-                // the state's part
-#pragma unroll
-                for (int x = 0; x < TILES; ++x) {
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) o[x][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int k = 0; k < STEPS; ++k) {
+                    for (int x = 0; x < TILES; ++x) {
                         f32x4_t lo = s[2 * k][x], hi = s[2 * k + 1][x];
                         const u32x2_t l1 = take_bf16(lo), h1 = take_bf16(hi);
                         const bf16x8_t one = pair(l1, h1);
                         const bf16x8_t two = pair(u32x2_t{f2bf2(lo[0], lo[1]), f2bf2(lo[2], lo[3])}, u32x2_t{f2bf2(hi[0], hi[1]), f2bf2(hi[2], hi[3])});
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            o[x][u] = product(one, qf[u][k], o[x][u]);
-                            o[x][u] = product(two, qf[u][k], o[x][u]);
-                        }
+                        for (int u = 0; u < 2; ++u) o[x][u] = product(one, qf[u], k == 0 ? zero : o[x][u]);
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) o[x][u] = product(two, qf[u], o[x][u]);
                     }
+                }
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
+                for (int x = 0; x < TILES; ++x) v[x] = read_values(x);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) o[x][u][r] *= since[u];
+                for (int u = 0; u < 2; ++u) {
+                    const float by = since[u] * faded;
+#pragma unroll
+                    for (int x = 0; x < TILES; ++x)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[x][u][r] *= by;
                 }
                 // the chunk's own
 #pragma unroll
@@ -380,23 +389,46 @@ __global__ void __launch_bounds__(kThreads, 2) k_linear_chunks(LinearArgs a) {
                     for (int x = 0; x < TILES; ++x) {
                         o[x][u] = product(v[x], one, o[x][u]);
                         o[x][u] = product(v[x], two, o[x][u]);
-                        done[x][u] = u32x2_t{f2bf2(o[x][u][0], o[x][u][1]), f2bf2(o[x][u][2], o[x][u][3])};
+                        done[u][2 * x] = f2bf2(o[x][u][0], o[x][u][1]);
+                        done[u][2 * x + 1] = f2bf2(o[x][u][2], o[x][u][3]);
                     }
                 }
+            } else {
+#pragma unroll
+                for (int x = 0; x < TILES; ++x) v[x] = read_values(x);
             }
+            __builtin_amdgcn_s_setprio(0);
+            if (j + 2 < chunks) load(j + 2);
             // the state behind the chunk
+            float more;   // by which what is added here counts in the accumulators
+            if (OUT) {
+                age += rows;
+                faded = __builtin_amdgcn_exp2f(rate * age);
+                more = 1.f;
+                if (faded < 0x1p-8f) {
+#pragma unroll
+                    for (int t = 0; t < DT; ++t)
+#pragma unroll
+                        for (int x = 0; x < TILES; ++x)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) s[t][x][r] *= faded;
+                    age = 0;
+                    faded = 1.f;
+                } else {
+                    more = __builtin_amdgcn_exp2f(-rate * age);
+                }
+            } else {
+                more = exp2f(rate * (j * kChunk));
+            }
             float weight[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) weight[e] = to_end[e];
-            Fade by = fade;
-            if (rows < kChunk) {
-                by = Fade(rows * log_decay);
+            for (int e = 0; e < 8; ++e) weight[e] = to_end[e] * more;
+            if (OUT && rows < kChunk)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int left = rows - 1 - ((e & 4) * 4 + 4 * g + (e & 3));
-                    weight[e] = left >= 0 ? exp2f(rate * left) : 0.f;
+                    weight[e] = left >= 0 ? exp2f(rate * left) * more : 0.f;
                 }
-            }
             bf16x8_t w[TILES][3];
 #pragma unroll
             for (int x = 0; x < TILES; ++x) {
@@ -417,23 +449,21 @@ __global__ void __launch_bounds__(kThreads, 2) k_linear_chunks(LinearArgs a) {
             }
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
-                const char* p = ki + (kt ^ (t * 2 * 16));
+                const char* p = ki + (kt ^ (t / 2 * 64)) + t % 2 * 8;
                 const bf16x8_t kf = __builtin_bit_cast(
                     bf16x8_t, __builtin_shufflevector(read_transposed(p), read_transposed(p + 16 * P * 16), 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                for (int x = 0; x < TILES; ++x) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s[t][x][r] = by(s[t][x][r]);
+                for (int x = 0; x < TILES; ++x)
 #pragma unroll
                     for (int z = 2; z >= 0; --z) s[t][x] = product(kf, w[x][z], s[t][x]);
-                }
             }
         }
         if (OUT && chunks > 0 && active) store(chunks - 1, count - (chunks - 1) * kChunk);
         float* end = nullptr;
-        if (!OUT) end = a.states + (bk * a.segments + segment + 1) * a.D * a.E;
+        if (!OUT) end = a.states + (bk * (1 + segments) + segment + 1) * a.D * a.E;
         else if (a.state_out && segment == last_segment && member == a.group - 1) end = a.state_out + bk * a.D * a.E;
         if (end) {
+            const Fade fade(age * log_decay);
             int here = lane;   // computed anew: the offsets of the first state's values would stay in registers through the loop
             asm volatile("" : "+v"(here));
 #pragma unroll
@@ -442,14 +472,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_linear_chunks(LinearArgs a) {
                 for (int x = 0; x < TILES; ++x)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int d = t * 16 + (here >> 4) * 4 + r, e = column + x * 16 + (here & 15);
-                        if (d < a.D && e < a.E) end[d * a.E + e] = s[t][x][r];
+                        const int d = t / 2 * 32 + (here >> 4) * 8 + t % 2 * 4 + r, e = column_of(x, here & 15);
+                        if (d < a.D && e < a.E) end[d * a.E + e] = fade(s[t][x][r]);
                     }
         }
         if (OUT) {   // the outputs behind the sequence
-            const int behind = max(n - first, 0), rows = min(a.N - first, a.length);
+            const int behind = max(n - first, 0), rows = min(a.N - first, length);
             const int pieces = a.E / 4;
-            for (int i = threadIdx.x; i < (rows - behind) * pieces; i += kThreads) {
+            for (int i = threadIdx.x; i < (rows - behind) * pieces; i += WAVES * 64) {
                 const int64_t row = row0 + behind + i / pieces;
                 *reinterpret_cast<uint2*>(a.out + row * a.ld_o + static_cast<int64_t>(head) * a.E + i % pieces * 4) = make_uint2(0, 0);
             }
@@ -463,23 +493,29 @@ __global__ void __launch_bounds__(kThreads, 2) k_linear_chunks(LinearArgs a) {
     }
 }
 
-// The segments' own states, each before the next one's place, become the states before them; the first is state_in or zeros.
+// From the pieces' own states to the state before each segment; the first is state_in or zeros.
 __global__ void __launch_bounds__(kThreads) k_linear_carry(LinearArgs a) {
+    constexpr int kAhead = 8;   // loads on their way: one at a time, 31 pieces took 17 us
     const int64_t size = static_cast<int64_t>(a.D) * a.E / 4, i = group_index() * kThreads + threadIdx.x;
     const int64_t bk = i / size;
     if (bk >= static_cast<int64_t>(a.B) * a.KH) return;
     const int64_t b = bk / a.KH;
-    const int n = a.lens ? min(max(a.lens[b], 0), a.N) : a.N, last = n > 0 ? (n - 1) / a.length : 0;
+    const int n = a.lens ? min(max(a.lens[b], 0), a.N) : a.N, last = n > 0 ? (n - 1) / (a.length * a.pieces) * a.pieces : 0;
     const Fade fade(static_cast<float>(a.length) * log_decay_of(a, static_cast<int>(bk % a.KH)));
     f32x4_t s = a.state_in ? reinterpret_cast<const f32x4_t*>(a.state_in)[i] : f32x4_t{0.f, 0.f, 0.f, 0.f};
-    f32x4_t* at = reinterpret_cast<f32x4_t*>(a.states) + bk * a.segments * size + (i - bk * size);
+    f32x4_t* at = reinterpret_cast<f32x4_t*>(a.states) + bk * (1 + (a.segments - 1) * a.pieces) * size + (i - bk * size);
     *at = s;
-    for (int m = 1; m <= last; ++m) {
-        at += size;
-        const f32x4_t own = *at;
+    for (int m = 1; m <= last; m += kAhead) {
+        f32x4_t own[kAhead];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[r] = fade(s[r]) + own[r];
-        *at = s;
+        for (int x = 0; x < kAhead; ++x) own[x] = at[min(m + x, last) * size];
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x)
+            if (m + x <= last) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[r] = fade(s[r]) + own[x][r];
+                if ((m + x) % a.pieces == 0) at[(m + x) * size] = s;
+            }
     }
 }
 
@@ -497,31 +533,65 @@ int device_cus() {
     return n;
 }
 
+// How a call runs: token after token for one or two (one 16 sequences of 32 heads of 128: 14.8 us against 19.0 for a chunk,
+// two 18.3 against 18.8, four 24.8 against 18.7), else chunks, each sequence in `segments`. The estimates, in us, were checked on
+// 15 shapes on one MI355X (1 to 512 heads of 64 to 128 columns, 128 to 32768 tokens), each in 1 to 64 segments: what they choose
+// is the fastest measured on 14, and 4% above it on 16 heads of 128 with 8192 tokens (16 segments 75, 32 72). A chunk
+// takes a workgroup `step` alone on a CU and 1.75 times that beside another; a call no less than its bytes at 4.6 TB/s;
+// the first launch 0.55 of a step a chunk; a state's load or store 30 us a MB for a workgroup, and the launch between
+// its states at 2.6 TB/s. One sequence each of 32 heads: 4 x 2048 tokens of 128 whole 150 us, in 4 segments 110, in 16 200;
+// 2 x 300 tokens of 64 heads of 64 whole 19, in 2 segments 23.
 struct Plan {
-    bool tokens;    // k_linear_tokens
-    int segments, length;
+    bool tokens;                    // k_linear_tokens
+    int segments, pieces, length;   // as in LinearArgs
 };
 Plan plan(const LinearShape& sh, bool may_split, int64_t cus) {
-    if (sh.seq_len <= 16) return Plan{true, 1, static_cast<int>(sh.seq_len)};
-    const int64_t chunks = (sh.seq_len + kChunk - 1) / kChunk, heads = sh.batch * sh.heads;
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(chunks / 4, (2 * cus + heads - 1) / heads));
-    const int64_t each = may_split ? (chunks + most - 1) / most : chunks;
-    return Plan{false, static_cast<int>((chunks + each - 1) / each), static_cast<int>(each * kChunk)};
+    if (sh.seq_len <= 2) return Plan{true, 1, 1, static_cast<int>(sh.seq_len)};
+    auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    const int64_t chunks = up(sh.seq_len, kChunk), heads = sh.batch * sh.heads, rows = sh.batch * sh.kv_heads;
+    // columns as the kernels compute them
+    const double width = static_cast<double>(up(sh.head_dim, 32) * 32 + (sh.value_dim > 64 ? 128 : 64)), step = 0.15 + 0.0082 * width;
+    const double state = 4e-6 * static_cast<double>(sh.head_dim * sh.value_dim);   // MB
+    const double bytes = 2.0 * static_cast<double>(sh.seq_len * (heads + rows) * (sh.head_dim + sh.value_dim));
+    auto rounds = [](double groups, double at_once) { return std::max(1.0, std::ceil(groups / at_once)); };
+    Plan best{false, 1, 1, static_cast<int>(chunks * kChunk)};
+    double least = 1e30;
+    for (int64_t want = 1; want == 1 || (may_split && want <= 512 && 2 * want <= chunks); want *= 2)
+        for (int64_t pieces = 1; pieces <= (want > 1 ? 2 : 1); ++pieces) {
+            const int64_t each = up(up(chunks, want), pieces) * pieces, segments = up(chunks, each);
+            const double groups = static_cast<double>(heads * segments), c = static_cast<double>(cus);
+            const double per = groups <= c ? step : 1.75 * step * rounds(groups, 2 * c);
+            double cost = 5 + std::max(each * per + std::max(1.0, groups / c) * state * 30, bytes / 4.6e6);
+            if (segments > 1) {
+                const double first = static_cast<double>(rows * (segments - 1) * pieces);
+                cost += 4 + each / pieces * 0.55 * step * (first <= c ? 1.0 : 0.8 * rounds(first, c)) + std::max(1.0, first / c) * state * 30;
+                cost += 3.5 + static_cast<double>(rows * segments * (pieces + 1)) * state / 2.6;
+            }
+            if (cost < least) {
+                least = cost;
+                best = Plan{false, static_cast<int>(segments), static_cast<int>(pieces), static_cast<int>(each / pieces * kChunk)};
+            }
+        }
+    return best;
 }
 
-template <int STEPS, int TILES, bool OUT>
+template <int STEPS, int TILES, int WAVES, bool OUT>
 void launch(const LinearArgs& a, int64_t groups, hipStream_t s) {
-    k_linear_chunks<STEPS, TILES, OUT><<<grid_of(groups, kThreads), kThreads, 0, s>>>(a);
+    k_linear_chunks<STEPS, TILES, WAVES, OUT><<<grid_of(groups, WAVES * 64), WAVES * 64, 0, s>>>(a);
     launch_check("attention_linear");
+}
+template <int STEPS, bool OUT>
+void by_values(const LinearArgs& a, int64_t groups, hipStream_t s) {
+    if (a.E > 64) launch<STEPS, 2, 4, OUT>(a, groups, s);
+    else launch<STEPS, 1, 4, OUT>(a, groups, s);
 }
 template <bool OUT>
 void by_width(const LinearArgs& a, int64_t groups, hipStream_t s) {
-    const bool wide = a.E > 64;
     switch ((a.D + 31) / 32) {
-        case 1: return wide ? launch<1, 2, OUT>(a, groups, s) : launch<1, 1, OUT>(a, groups, s);
-        case 2: return wide ? launch<2, 2, OUT>(a, groups, s) : launch<2, 1, OUT>(a, groups, s);
-        case 3: return wide ? launch<3, 2, OUT>(a, groups, s) : launch<3, 1, OUT>(a, groups, s);
-        default: return wide ? launch<4, 2, OUT>(a, groups, s) : launch<4, 1, OUT>(a, groups, s);
+        case 1: return by_values<1, OUT>(a, groups, s);
+        case 2: return by_values<2, OUT>(a, groups, s);
+        case 3: return by_values<3, OUT>(a, groups, s);
+        default: return by_values<4, OUT>(a, groups, s);
     }
 }
 
@@ -531,7 +601,7 @@ int64_t attention_linear_workspace_floats(const LinearShape& sh) {
     const Plan how = plan(sh, true, device_cus());
     const int64_t states = sh.batch * sh.kv_heads * sh.head_dim * sh.value_dim;
     // one state each where a group's heads would still read what one of them writes
-    return how.segments > 1 ? how.segments * states : !how.tokens && sh.heads > sh.kv_heads ? states : 0;
+    return how.segments > 1 ? (1 + (how.segments - 1) * how.pieces) * states : !how.tokens && sh.heads > sh.kv_heads ? states : 0;
 }
 
 bh_attention_linear_plan attention_linear_plan(const LinearShape& sh, bool may_split, int cus) {
@@ -556,6 +626,7 @@ void launch_attention_linear(const bf16_t* q, const bf16_t* k, const bf16_t* v, 
     const Plan how = plan(sh, ws != nullptr, device_cus());
     a.states = ws;
     a.segments = how.segments;
+    a.pieces = how.pieces;
     a.length = how.length;
     ProfileScope ps(K_ATTN_SELF, s, 2.0 * sh.batch * sh.seq_len * (sh.heads + sh.kv_heads) * sh.head_dim * sh.value_dim);
     const int64_t rows = sh.batch * sh.kv_heads;
@@ -570,8 +641,8 @@ void launch_attention_linear(const bf16_t* q, const bf16_t* k, const bf16_t* v, 
     a.first_state = copied ? 2 : state_in ? 1 : 0;
     a.heads_each = in_place && !copied ? a.group : 1;
     const int64_t groups = rows * how.segments * (a.group / a.heads_each);
-    require(groups < (int64_t{1} << 40), "attention_linear: too many heads");
-    if (how.segments > 1) by_width<false>(a, rows * (how.segments - 1), s);
+    require(groups < (int64_t{1} << 31), "attention_linear: too many heads");
+    if (how.segments > 1) by_width<false>(a, rows * (how.segments - 1) * how.pieces, s);
     if (copied) {
         k_linear_carry<<<grid_of((rows * a.D * a.E / 4 + kThreads - 1) / kThreads, kThreads), kThreads, 0, s>>>(a);
         launch_check("attention_linear");
