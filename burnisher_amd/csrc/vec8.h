@@ -38,6 +38,37 @@ __device__ __forceinline__ void load8(const T* p, int64_t col, int64_t cols, flo
     for (int e = 0; e < 8; ++e) v[e] = col + e < cols ? value(p[e]) : 0.0f;
 }
 
+// Eight values as they lie in memory until they are used (four registers of bf16, eight of fp32), at any alignment.
+template <typename T>
+struct Packed8 {
+    static constexpr int kWords = sizeof(T) == 2 ? 4 : 8;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load(const T* p) {
+        typedef u32x4_t Any __attribute__((aligned(2)));
+#pragma unroll
+        for (int i = 0; i < kWords / 4; ++i) {
+            const u32x4_t r = reinterpret_cast<const Any*>(p)[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[4 * i + e] = r[e];
+        }
+    }
+    // The last 8 - skip of a row of fewer than eight values, p where the first would be.
+    __device__ __forceinline__ void load_from(const T* p, int skip) {
+        uint32_t bits[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (sizeof(T) == 2) bits[e] = e >= skip ? p[e] : 0u;
+            else bits[e] = e >= skip ? __float_as_uint(p[e]) : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = sizeof(T) == 2 ? bits[2 * i % 8] | bits[(2 * i + 1) % 8] << 16 : bits[i];
+    }
+    __device__ __forceinline__ float operator[](int e) const {
+        if constexpr (sizeof(T) == 2) return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+        else return __uint_as_float(w[e]);
+    }
+};
+
 // Those of columns below `cols`, each rounded once.
 template <typename T>
 __device__ __forceinline__ void store8(T* p, int64_t col, int64_t cols, const float (&v)[8]) {
