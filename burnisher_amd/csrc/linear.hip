@@ -168,16 +168,23 @@ __device__ __forceinline__ bf16x8_t pair(u32x2_t x, u32x2_t y) {
 __device__ __forceinline__ f32x4_t product(bf16x8_t a, bf16x8_t b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-// The bf16 nearest to each value, and what is left of the values.
-__device__ __forceinline__ u32x2_t take_bf16(f32x4_t& v) {
-    u32x2_t h = {f2bf2(v[0], v[1]), f2bf2(v[2], v[3])};
-    asm("" : "+v"(h));   // one conversion: the compiler would convert each value again to get it alone
-    v[0] -= __uint_as_float(h[0] << 16);
-    v[1] -= __uint_as_float(h[0] & 0xffff0000u);
-    v[2] -= __uint_as_float(h[1] << 16);
-    v[3] -= __uint_as_float(h[1] & 0xffff0000u);
-    return h;
-}
+// The bf16 nearest to each value, and what is left of the values: v - h as v + (h, h') . (-1, 0), the dot product of a pair,
+// exact here (h is within a factor of two of v), which takes h from its pair as it is.
+struct Split {
+    uint32_t first, second;   // (-1, 0) and (0, -1); opaque, since an inline -1 would stand for the second
+    __device__ __forceinline__ Split() : first(0x0000bf80u), second(0xbf800000u) { asm volatile("" : "+s"(first), "+s"(second)); }
+    __device__ __forceinline__ u32x2_t operator()(f32x4_t& v) const {
+        u32x2_t h = {f2bf2(v[0], v[1]), f2bf2(v[2], v[3])};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t word = h[i];   // a value: the cast of a vector's element takes its first
+            const bf16x2_t p = __builtin_bit_cast(bf16x2_t, word);
+            v[2 * i] = __builtin_amdgcn_fdot2_f32_bf16(p, __builtin_bit_cast(bf16x2_t, first), v[2 * i], false);
+            v[2 * i + 1] = __builtin_amdgcn_fdot2_f32_bf16(p, __builtin_bit_cast(bf16x2_t, second), v[2 * i + 1], false);
+        }
+        return h;
+    }
+};
 
 // STEPS: of 32 columns of q and k; TILES: of 16 value columns a wave. With OUT a workgroup walks a segment for one query
 // head from the state before it. Without, it adds up a piece's own state from k and v, from its end back, so that
@@ -233,6 +240,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
     const int vt = TILES == 2 ? trow * PV * 16 + ((c & 3) ^ turn<PV, 2>(trow)) * 16
                               : trow * PV * 16 + (((c & 3) >> 1) ^ turn<PV, 1>(trow)) * 16 + (c & 1) * 8;
 
+    const Split take_bf16;
     // powers of the decay: token j of the fragment's order before the chunk's end, and (times scale) query c of a tile
     // against the keys of its own tile, of the one before, and the state
     float to_end[8], own[4], before[4], since[2];
@@ -317,21 +325,32 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
             else s_waitcnt<0, 0>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            if (OUT && j > 0) store(j - 1, kChunk);
-            if (!active) {
-                if (j + 2 < chunks) load(j + 2);
-                continue;
-            }
             const int rows = min(count - j * kChunk, kChunk);
             const char* image = smem + j % kStages * kStage;
             const char *qi = image, *ki = image + kLoadsQ * 1024, *vi = ki + kLoadsK * 1024;
-
+            auto read_keys = [&](int t) {   // transposed
+                const char* p = ki + (kt ^ (t / 2 * 64)) + t % 2 * 8;
+                return __builtin_bit_cast(
+                    bf16x8_t, __builtin_shufflevector(read_transposed(p), read_transposed(p + 16 * P * 16), 0, 1, 2, 3, 4, 5, 6, 7));
+            };
             auto read_values = [&](int x) {
                 const char* p = vi + (vt ^ (column / 8 * 16)) + x * 8;
                 return __builtin_bit_cast(
                     bf16x8_t, __builtin_shufflevector(read_transposed(p), read_transposed(p + 16 * PV * 16), 0, 1, 2, 3, 4, 5, 6, 7));
             };
-            bf16x8_t v[TILES];
+            if (OUT && j > 0) store(j - 1, kChunk);
+            if (!active) {
+                if (j + 2 < chunks) load(j + 2);
+                continue;
+            }
+            // the transposed operands are read ahead of what comes before them: 8 x 2048 tokens of 32 heads of 64 74 us instead of 77
+            bf16x8_t v[TILES], keys[2][2];   // keys: [pair of tiles % 2][tile]
+            auto read_first = [&]() {
+#pragma unroll
+                for (int x = 0; x < TILES; ++x) v[x] = read_values(x);
+#pragma unroll
+                for (int y = 0; y < 2; ++y) keys[0][y] = read_keys(y);
+            };
             if (OUT) {
                 // by 32 rows of the state: scores of key tile y against query tile u >= y, and the state's part of the outputs
                 const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
@@ -339,17 +358,18 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
                 f32x4_t o[TILES][2], score[3];   // (0, 0), (0, 1), (1, 1)
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
-                    bf16x8_t qf[2], kf[2];
+                    bf16x8_t q[2], kk[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         u32x4_t f = *reinterpret_cast<const u32x4_t*>(qi + u * 16 * P * 16 + (frag ^ (k * 64)));
                         if (k == STEPS - 1 && k * 4 + g >= dc) f = u32x4_t{0, 0, 0, 0};   // past head_dim
-                        qf[u] = __builtin_bit_cast(bf16x8_t, f);
-                        kf[u] = *reinterpret_cast<const bf16x8_t*>(ki + u * 16 * P * 16 + (frag ^ (k * 64)));
+                        q[u] = __builtin_bit_cast(bf16x8_t, f);
+                        kk[u] = *reinterpret_cast<const bf16x8_t*>(ki + u * 16 * P * 16 + (frag ^ (k * 64)));
                     }
-                    score[0] = product(kf[0], qf[0], k == 0 ? zero : score[0]);
-                    score[1] = product(kf[0], qf[1], k == 0 ? zero : score[1]);
-                    score[2] = product(kf[1], qf[1], k == 0 ? zero : score[2]);
+                    if (k + 1 == STEPS) read_first();
+                    score[0] = product(kk[0], q[0], k == 0 ? zero : score[0]);
+                    score[1] = product(kk[0], q[1], k == 0 ? zero : score[1]);
+                    score[2] = product(kk[1], q[1], k == 0 ? zero : score[2]);
 #pragma unroll
                     for (int x = 0; x < TILES; ++x) {
                         f32x4_t lo = s[2 * k][x], hi = s[2 * k + 1][x];
@@ -357,13 +377,11 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
                         const bf16x8_t one = pair(l1, h1);
                         const bf16x8_t two = pair(u32x2_t{f2bf2(lo[0], lo[1]), f2bf2(lo[2], lo[3])}, u32x2_t{f2bf2(hi[0], hi[1]), f2bf2(hi[2], hi[3])});
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) o[x][u] = product(one, qf[u], k == 0 ? zero : o[x][u]);
+                        for (int u = 0; u < 2; ++u) o[x][u] = product(one, q[u], k == 0 ? zero : o[x][u]);
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) o[x][u] = product(two, qf[u], o[x][u]);
+                        for (int u = 0; u < 2; ++u) o[x][u] = product(two, q[u], o[x][u]);
                     }
                 }
-#pragma unroll
-                for (int x = 0; x < TILES; ++x) v[x] = read_values(x);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const float by = since[u] * faded;
@@ -394,8 +412,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
                     }
                 }
             } else {
-#pragma unroll
-                for (int x = 0; x < TILES; ++x) v[x] = read_values(x);
+                read_first();
             }
             __builtin_amdgcn_s_setprio(0);
             if (j + 2 < chunks) load(j + 2);
@@ -448,14 +465,16 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
                 }
             }
 #pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                const char* p = ki + (kt ^ (t / 2 * 64)) + t % 2 * 8;
-                const bf16x8_t kf = __builtin_bit_cast(
-                    bf16x8_t, __builtin_shufflevector(read_transposed(p), read_transposed(p + 16 * P * 16), 0, 1, 2, 3, 4, 5, 6, 7));
+            for (int k = 0; k < STEPS; ++k) {
+                if (k + 1 < STEPS)
 #pragma unroll
-                for (int x = 0; x < TILES; ++x)
+                    for (int y = 0; y < 2; ++y) keys[(k + 1) & 1][y] = read_keys(2 * k + 2 + y);
 #pragma unroll
-                    for (int z = 2; z >= 0; --z) s[t][x] = product(kf, w[x][z], s[t][x]);
+                for (int z = 2; z >= 0; --z)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+#pragma unroll
+                        for (int x = 0; x < TILES; ++x) s[2 * k + y][x] = product(keys[k & 1][y], w[x][z], s[2 * k + y][x]);
             }
         }
         if (OUT && chunks > 0 && active) store(chunks - 1, count - (chunks - 1) * kChunk);
