@@ -660,7 +660,7 @@ void launch_attention_linear(const bf16_t* q, const bf16_t* k, const bf16_t* v, 
     a.first_state = copied ? 2 : state_in ? 1 : 0;
     a.heads_each = in_place && !copied ? a.group : 1;
     const int64_t groups = rows * how.segments * (a.group / a.heads_each);
-    require(groups < (int64_t{1} << 31), "attention_linear: too many heads");
+    require(groups < (int64_t{1} << 31) && rows * how.segments * how.pieces < (int64_t{1} << 31), "attention_linear: too many heads");
     if (how.segments > 1) by_width<false>(a, rows * (how.segments - 1) * how.pieces, s);
     if (copied) {
         k_linear_carry<<<grid_of((rows * a.D * a.E / 4 + kThreads - 1) / kThreads, kThreads), kThreads, 0, s>>>(a);
