@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
 
 // From the pieces' own states to the state before each segment; the first is state_in or zeros.
 __global__ void __launch_bounds__(kThreads) k_linear_carry(LinearArgs a) {
-    constexpr int kAhead = 8;   // loads on their way: one at a time, 31 pieces took 17 us
+    constexpr int kAhead = 16;   // loads on their way: with 8, 255 pieces of one head of 128 took 13 us longer
     const int64_t size = static_cast<int64_t>(a.D) * a.E / 4, i = group_index() * kThreads + threadIdx.x;
     const int64_t bk = i / size;
     if (bk >= static_cast<int64_t>(a.B) * a.KH) return;
@@ -552,14 +552,14 @@ int device_cus() {
     return n;
 }
 
-// How a call runs: token after token for one or two (one 16 sequences of 32 heads of 128: 14.8 us against 19.0 for a chunk,
+// How a call runs: token after token for one or two (one token of 16 sequences, 32 heads of 128: 14.8 us against 19.0 for a chunk,
 // two 18.3 against 18.8, four 24.8 against 18.7), else chunks, each sequence in `segments`. The estimates, in us, were checked on
-// 15 shapes on one MI355X (1 to 512 heads of 64 to 128 columns, 128 to 32768 tokens), each in 1 to 64 segments: what they choose
-// is the fastest measured on 14, and 4% above it on 16 heads of 128 with 8192 tokens (16 segments 75, 32 72). A chunk
-// takes a workgroup `step` alone on a CU and 1.75 times that beside another; a call no less than its bytes at 4.6 TB/s;
-// the first launch 0.55 of a step a chunk; a state's load or store 30 us a MB for a workgroup, and the launch between
-// its states at 2.6 TB/s. One sequence each of 32 heads: 4 x 2048 tokens of 128 whole 150 us, in 4 segments 110, in 16 200;
-// 2 x 300 tokens of 64 heads of 64 whole 19, in 2 segments 23.
+// 26 shapes on one MI355X (1 to 256 heads of 32 to 128 columns, 256 to 65536 tokens), each in 1 to 256 segments: what they choose
+// is within 7% of the fastest measured on 25, and 10% above it on 4 x 1024 tokens of 32 heads of 128 (73 whole, 67 in 2). A chunk takes a workgroup `step` alone on a CU, and
+// beside others the CU `share` of that for each; a call no less than its bytes at 4.6 TB/s; the first launch 0.55 of a step
+// a chunk; a state's load or store 30 us a MB for a workgroup, and the launch between its states at 2.6 TB/s and 0.08
+// a piece. 4 x 2048 tokens of 32 heads of 128 whole 137 us, in 4 segments 107, in 16 208; one head of 128 with 8192 tokens
+// whole 523, in 64 segments 37, in 256 62; 2 x 300 tokens of 64 heads of 64 whole 16.5, in 2 segments 23.
 struct Plan {
     bool tokens;                    // k_linear_tokens
     int segments, pieces, length;   // as in LinearArgs
@@ -569,22 +569,22 @@ Plan plan(const LinearShape& sh, bool may_split, int64_t cus) {
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     const int64_t chunks = up(sh.seq_len, kChunk), heads = sh.batch * sh.heads, rows = sh.batch * sh.kv_heads;
     // columns as the kernels compute them
-    const double width = static_cast<double>(up(sh.head_dim, 32) * 32 + (sh.value_dim > 64 ? 128 : 64)), step = 0.15 + 0.0082 * width;
+    const double width = static_cast<double>(up(sh.head_dim, 32) * 32 + (sh.value_dim > 64 ? 128 : 64));
+    const double step = 0.1 + 0.0078 * width, share = width >= 192 ? 0.8 : 0.5;
     const double state = 4e-6 * static_cast<double>(sh.head_dim * sh.value_dim);   // MB
     const double bytes = 2.0 * static_cast<double>(sh.seq_len * (heads + rows) * (sh.head_dim + sh.value_dim));
-    auto rounds = [](double groups, double at_once) { return std::max(1.0, std::ceil(groups / at_once)); };
     Plan best{false, 1, 1, static_cast<int>(chunks * kChunk)};
     double least = 1e30;
     for (int64_t want = 1; want == 1 || (may_split && want <= 512 && 2 * want <= chunks); want *= 2)
         for (int64_t pieces = 1; pieces <= (want > 1 ? 2 : 1); ++pieces) {
             const int64_t each = up(up(chunks, want), pieces) * pieces, segments = up(chunks, each);
             const double groups = static_cast<double>(heads * segments), c = static_cast<double>(cus);
-            const double per = groups <= c ? step : 1.75 * step * rounds(groups, 2 * c);
+            const double per = step * std::max(1.0, share * std::ceil(groups / c));
             double cost = 5 + std::max(each * per + std::max(1.0, groups / c) * state * 30, bytes / 4.6e6);
             if (segments > 1) {
-                const double first = static_cast<double>(rows * (segments - 1) * pieces);
-                cost += 4 + each / pieces * 0.55 * step * (first <= c ? 1.0 : 0.8 * rounds(first, c)) + std::max(1.0, first / c) * state * 30;
-                cost += 3.5 + static_cast<double>(rows * segments * (pieces + 1)) * state / 2.6;
+                const double first = static_cast<double>(rows * (segments - 1) * pieces), all = static_cast<double>(segments * pieces);
+                cost += 3 + each / pieces * 0.55 * step * std::max(1.0, share * std::ceil(first / c)) + std::max(1.0, first / c) * state * 30;
+                cost += 3.5 + 0.08 * all + static_cast<double>(rows) * (all + segments) * state / 2.6;
             }
             if (cost < least) {
                 least = cost;
