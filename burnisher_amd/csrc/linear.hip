@@ -570,7 +570,7 @@ Plan plan(const LinearShape& sh, bool may_split, int64_t cus) {
     const int64_t chunks = up(sh.seq_len, kChunk), heads = sh.batch * sh.heads, rows = sh.batch * sh.kv_heads;
     // columns as the kernels compute them
     const double width = static_cast<double>(up(sh.head_dim, 32) * 32 + (sh.value_dim > 64 ? 128 : 64));
-    const double step = 0.1 + 0.0078 * width, share = width >= 192 ? 0.8 : 0.5;
+    const double step = 0.1 + 0.0078 * width, share = width >= 192 ? 0.8 : 0.5, alone = sh.value_dim > 64 ? 0.9 : 1.0;
     const double state = 4e-6 * static_cast<double>(sh.head_dim * sh.value_dim);   // MB
     const double bytes = 2.0 * static_cast<double>(sh.seq_len * (heads + rows) * (sh.head_dim + sh.value_dim));
     Plan best{false, 1, 1, static_cast<int>(chunks * kChunk)};
@@ -579,7 +579,7 @@ Plan plan(const LinearShape& sh, bool may_split, int64_t cus) {
         for (int64_t pieces = 1; pieces <= (want > 1 ? 2 : 1); ++pieces) {
             const int64_t each = up(up(chunks, want), pieces) * pieces, segments = up(chunks, each);
             const double groups = static_cast<double>(heads * segments), c = static_cast<double>(cus);
-            const double per = step * std::max(1.0, share * std::ceil(groups / c));
+            const double per = step * (groups <= c ? alone : std::max(1.0, share * std::ceil(groups / c)));
             double cost = 5 + std::max(each * per + std::max(1.0, groups / c) * state * 30, bytes / 4.6e6);
             if (segments > 1) {
                 const double first = static_cast<double>(rows * (segments - 1) * pieces), all = static_cast<double>(segments * pieces);
@@ -599,18 +599,22 @@ void launch(const LinearArgs& a, int64_t groups, hipStream_t s) {
     k_linear_chunks<STEPS, TILES, WAVES, OUT><<<grid_of(groups, WAVES * 64), WAVES * 64, 0, s>>>(a);
     launch_check("attention_linear");
 }
+// More than 64 value columns to four waves of 32, or where a workgroup has its CU to itself to eight of 16, which take a chunk in
+// 0.9 of the time (8 heads of 128 with 100 tokens 16.3 us against 18.0) and two workgroups' chunks in 1.2 of it.
 template <int STEPS, bool OUT>
-void by_values(const LinearArgs& a, int64_t groups, hipStream_t s) {
-    if (a.E > 64) launch<STEPS, 2, 4, OUT>(a, groups, s);
-    else launch<STEPS, 1, 4, OUT>(a, groups, s);
+void by_values(const LinearArgs& a, int64_t groups, int64_t cus, hipStream_t s) {
+    if (a.E <= 64) return launch<STEPS, 1, 4, OUT>(a, groups, s);
+    if constexpr (OUT)
+        if (groups <= cus) return launch<STEPS, 1, 8, OUT>(a, groups, s);
+    launch<STEPS, 2, 4, OUT>(a, groups, s);
 }
 template <bool OUT>
-void by_width(const LinearArgs& a, int64_t groups, hipStream_t s) {
+void by_width(const LinearArgs& a, int64_t groups, int64_t cus, hipStream_t s) {
     switch ((a.D + 31) / 32) {
-        case 1: return by_values<1, OUT>(a, groups, s);
-        case 2: return by_values<2, OUT>(a, groups, s);
-        case 3: return by_values<3, OUT>(a, groups, s);
-        default: return by_values<4, OUT>(a, groups, s);
+        case 1: return by_values<1, OUT>(a, groups, cus, s);
+        case 2: return by_values<2, OUT>(a, groups, cus, s);
+        case 3: return by_values<3, OUT>(a, groups, cus, s);
+        default: return by_values<4, OUT>(a, groups, cus, s);
     }
 }
 
@@ -642,7 +646,8 @@ void launch_attention_linear(const bf16_t* q, const bf16_t* k, const bf16_t* v, 
     a.N = static_cast<int>(sh.seq_len); a.D = static_cast<int>(sh.head_dim); a.E = static_cast<int>(sh.value_dim);
     a.slices = (a.E + 31) / 32;
     a.scale = sh.scale;
-    const Plan how = plan(sh, ws != nullptr, device_cus());
+    const int64_t cus = device_cus();
+    const Plan how = plan(sh, ws != nullptr, cus);
     a.states = ws;
     a.segments = how.segments;
     a.pieces = how.pieces;
@@ -661,12 +666,12 @@ void launch_attention_linear(const bf16_t* q, const bf16_t* k, const bf16_t* v, 
     a.heads_each = in_place && !copied ? a.group : 1;
     const int64_t groups = rows * how.segments * (a.group / a.heads_each);
     require(groups < (int64_t{1} << 31) && rows * how.segments * how.pieces < (int64_t{1} << 31), "attention_linear: too many heads");
-    if (how.segments > 1) by_width<false>(a, rows * (how.segments - 1) * how.pieces, s);
+    if (how.segments > 1) by_width<false>(a, rows * (how.segments - 1) * how.pieces, cus, s);
     if (copied) {
         k_linear_carry<<<grid_of((rows * a.D * a.E / 4 + kThreads - 1) / kThreads, kThreads), kThreads, 0, s>>>(a);
         launch_check("attention_linear");
     }
-    by_width<true>(a, groups, s);
+    by_width<true>(a, groups, cus, s);
 }
 
 }  // namespace bh
