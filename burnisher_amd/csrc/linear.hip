@@ -18,10 +18,10 @@
 // from k and v, a second runs over the segments' states, and in a third each segment starts from its own.
 //
 // What bounds it: one token of 16 sequences, 32 states of 128 x 128 each, their bytes (14.9 us, 4.5 TB/s). Chunks, the
-// instructions of few waves: at 128 x 128 a chunk takes 2.2 us alone on a CU, two 4.0, where matrix (1600 cycles) and vector
-// instructions (310, and address work) of two waves of a SIMD overlap little, and issuing the 24 direct loads takes 600 to 900.
-// 2 x 4096 tokens of 32 / 8 heads of 128 83 us, 64 of it the third launch; 65536 tokens of 16 heads of 128 356 us, near its
-// bytes: k and v twice, 108 us of it the first launch (5.0 TB/s), 15 the second; 2 x 300 of 64 heads of 64 16.6 us.
+// instructions of few waves: at 128 x 128 a chunk takes 2.3 us alone on a CU, two 3.9, where matrix (100, 1600 cycles) and vector
+// instructions (361) of two waves of a SIMD overlap little, and issuing a wave's six direct loads takes 500 to 800 cycles of 6500.
+// 2 x 4096 tokens of 32 / 8 heads of 128 83 us, 65 of it the third launch; 65536 tokens of 16 heads of 128 356 us, near its
+// bytes: k and v twice, 108 us of it the first launch (4.8 TB/s), 15 the second; 2 x 300 of 64 heads of 64 16.6 us.
 #include "common.h"
 
 #include <algorithm>
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
                 }
 
         // The state is `faded` times what the accumulators hold: its decay is put off, as a factor of what is added, until
-        // it comes to 2^-8 since `age` tokens. Applied in every chunk it took 128 of 650 vector instructions.
+        // it comes to 2^-8 since `age` tokens. Applied in every chunk it took 128 of 662 vector instructions.
         int age = 0;
         float faded = 1.f;
         typedef uint32_t out_t __attribute__((ext_vector_type(2 * TILES)));
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
             if (OUT) {
                 // by 32 rows of the state: scores of key tile y against query tile u >= y, and the state's part of the outputs
                 const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-                __builtin_amdgcn_s_setprio(1);
+                __builtin_amdgcn_s_setprio(1);   // before the other wave's loads and values: 2 x 4096 tokens of 32 / 8 heads of 128 84 us, without 88
                 f32x4_t o[TILES][2], score[3];   // (0, 0), (0, 1), (1, 1)
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {

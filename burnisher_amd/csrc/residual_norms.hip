@@ -6,7 +6,7 @@
 // second norm before it is rounded.
 //
 // Bound by HBM for wide rows (4096 x 4096 bf16: 29 us, 4.6 TB/s); rows of 1152 columns with gate, scale and shift, 8192 of them
-// in 17.6 us (4.3 TB/s), are bound by vector instructions too, some 40 an element, which is why a row's address and a
+// in 17.6 us (4.3 TB/s), are bound by vector instructions too, 45 an element, which is why a row's address and a
 // modulation's row are scalar and no lane has a path of its own. One row of 4096: 3.4 us, a launch.
 #include "common.h"
 #include "vec8.h"
