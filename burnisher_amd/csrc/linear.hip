@@ -50,7 +50,7 @@ struct LinearArgs {
     float* states;
     int segments, pieces, length;   // of a sequence, of a segment, tokens of a piece (a multiple of kChunk)
     int first_state;        // the first segment's: 0 zeros, 1 state_in, 2 states
-    int heads_each;         // query heads that a workgroup takes one after the other: 1, or the group
+    int turns;              // that a workgroup takes its query heads in, one after the other: 1, or enough for the group
     float scale;
 };
 
@@ -137,11 +137,9 @@ __global__ void __launch_bounds__(kThreads) k_linear_tokens(LinearArgs a) {
 // ---- chunks ------------------------------------------------------------------------------------------
 
 constexpr int kChunk = 32;
-constexpr int kStages = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
-typedef short s16x8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
@@ -192,18 +190,22 @@ struct Split {
     }
 };
 
-// STEPS: of 32 columns of q and k; TILES: of 16 value columns a wave. With OUT a workgroup walks a segment for one query
-// head from the state before it. Without, it adds up a piece's own state from k and v, from its end back, so that
-// weights only fall and the walk ends where they are zero, and what it read last is what the next launch reads first.
-template <int STEPS, int TILES, int WAVES, bool OUT>
+// STEPS: of 32 columns of q and k; TILES: of 16 value columns a wave. A workgroup walks a segment from the state before it
+// for HEADS query heads of a group at once, which have the state in common. With none it adds up a piece's own state from
+// k and v, from its end back, so that weights only fall and the walk ends where they are zero, and what it read last is
+// what the next launch reads first.
+template <int STEPS, int TILES, int WAVES, int HEADS>
 __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
     constexpr int P = places(STEPS), PV = places(WAVES * TILES / 2), DT = 2 * STEPS;
-    constexpr int kLoadsQ = OUT ? P / 2 : 0, kLoadsK = P / 2, kLoads = kLoadsQ + kLoadsK + PV / 2;   // of 1 KiB
+    constexpr bool OUT = HEADS > 0;
+    constexpr int kLoadsQ = HEADS * (P / 2), kLoadsK = P / 2, kLoads = kLoadsQ + kLoadsK + PV / 2;   // of 1 KiB
     constexpr int kItems = (kLoads + WAVES - 1) / WAVES;                                             // a wave's
-    constexpr int kStage = kLoads * 1024;
+    // Two workgroups fit a CU. Two stages instead of three: 4 x 2400 tokens of 64 heads of 64, one workgroup a CU, 108 us for 85, but
+    // 2 x 300 15.9 for 16.9 and 8 x 2400 147 for 163. Two heads of 128 at once in three stages, alone on a CU, lost 4 to 10%.
+    constexpr int kStage = kLoads * 1024, kStages = 3 * kStage <= 80 * 1024 ? 3 : 2;
     __shared__ __attribute__((aligned(1024))) char smem[kStages * kStage];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-    const int per = OUT ? a.group / a.heads_each : 1, segments = OUT ? a.segments : (a.segments - 1) * a.pieces;
+    const int per = OUT ? a.group / (HEADS * a.turns) : 1, segments = OUT ? a.segments : (a.segments - 1) * a.pieces;
     const int64_t number = group_index();
     const int T = a.B * a.KH * segments * per;
     if (number >= T) return;
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
     const uint32_t ldq = static_cast<uint32_t>(a.ld_q) * 2, ldk = static_cast<uint32_t>(a.ld_k) * 2, ldv = static_cast<uint32_t>(a.ld_v) * 2;
     const int dc = a.D / 8, ec = a.E / 8;
     auto offset = [&](int m, int last_row) {
-        return m < kLoadsQ             ? source<P, 2>(m, lane, dc, last_row, ldq)
+        return m < kLoadsQ             ? source<P, 2>(m % (P / 2), lane, dc, last_row, ldq)
                : m < kLoadsQ + kLoadsK ? source<P, 2>(m - kLoadsQ, lane, dc, last_row, ldk)
                                        : source<PV, TILES>(m - kLoadsQ - kLoadsK, lane, ec, last_row, ldv);
     };
@@ -261,15 +263,15 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) since[u] = exp2f(rate * (16 * u + c + 1)) * a.scale;
 
-    for (int turn_of = 0; turn_of < (OUT ? a.heads_each : 1); ++turn_of) {
-        const int member = at + turn_of, head = kh * a.group + member;
+    for (int turn_of = 0; turn_of < (OUT ? a.turns : 1); ++turn_of) {
+        const int member = (at + turn_of) * HEADS, head = kh * a.group + member;   // the first
         const bf16_t* q0 = OUT ? a.q + row0 * a.ld_q + static_cast<int64_t>(head) * a.D : nullptr;
         auto load = [&](int j) {
             const int64_t t = OUT ? j * kChunk : length - (j + 1) * kChunk;
             const int rows = OUT ? count - j * kChunk : kChunk;
             const bf16_t *q = q0 + t * a.ld_q, *k = k0 + t * a.ld_k, *v = v0 + t * a.ld_v;
             const char* to = smem + j % kStages * kStage;
-            auto from = [&](int m) { return m < kLoadsQ ? q : m < kLoadsQ + kLoadsK ? k : v; };
+            auto from = [&](int m) { return m < kLoadsQ ? q + m / (P / 2) * a.D : m < kLoadsQ + kLoadsK ? k : v; };
             if (rows >= kChunk) {
 #pragma unroll
                 for (int i = 0; i < kItems; ++i) {
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
             }
         };
         if (chunks > 0) load(0);
-        if (chunks > 1) load(1);
+        if (kStages == 3 && chunks > 1) load(1);
 
         // s[t][x][r]: row 32 (t / 2) + 8 g + 4 (t % 2) + r, column column_of(x, c)
         f32x4_t s[DT][TILES];
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
         int age = 0;
         float faded = 1.f;
         typedef uint32_t out_t __attribute__((ext_vector_type(2 * TILES)));
-        out_t done[2];   // the last chunk's outputs, columns column_of(0, 4 g) on of query c: they leave behind the next barrier
+        out_t done[OUT ? HEADS : 1][2];   // the last chunk's outputs, columns column_of(0, 4 g) on of query c: they leave behind the next barrier
         auto store = [&](int j, int rows) {
             const int e = column_of(0, g * 4);
 #pragma unroll
@@ -320,14 +322,16 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
                 const int i = u * 16 + c;
                 typedef out_t Any __attribute__((aligned(8)));
                 if (e < a.E && i < rows)
-                    *reinterpret_cast<Any*>(a.out + (row0 + j * kChunk + i) * a.ld_o + static_cast<int64_t>(head) * a.E + e) = done[u];
+#pragma unroll
+                    for (int h = 0; h < HEADS; ++h)
+                        *reinterpret_cast<Any*>(a.out + (row0 + j * kChunk + i) * a.ld_o + static_cast<int64_t>(head + h) * a.E + e) = done[h][u];
             }
         };
         for (int j = 0; j < chunks; ++j) {
             // this wave's loads of chunk j have landed, those of chunk j + 1 may be on their way; behind the barrier
             // everyone's have, and chunk j - 1 has been read
             asm volatile("" ::: "memory");
-            if (j + 1 < chunks) s_waitcnt<kItems, 0>();
+            if (kStages == 3 && j + 1 < chunks) s_waitcnt<kItems, 0>();
             else s_waitcnt<0, 0>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
@@ -346,7 +350,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
             };
             if (OUT && j > 0) store(j - 1, kChunk);
             if (!active) {
-                if (j + 2 < chunks) load(j + 2);
+                if (j + kStages - 1 < chunks) load(j + kStages - 1);
                 continue;
             }
             // the transposed operands are read ahead of what comes before them: 8 x 2048 tokens of 32 heads of 64 74 us instead of 77
@@ -357,25 +361,31 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
 #pragma unroll
                 for (int y = 0; y < 2; ++y) keys[0][y] = read_keys(y);
             };
-            if (OUT) {
+            if constexpr (OUT) {
                 // by 32 rows of the state: scores of key tile y against query tile u >= y, and the state's part of the outputs
                 const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
                 __builtin_amdgcn_s_setprio(1);   // before the other wave's loads and values: 2 x 4096 tokens of 32 / 8 heads of 128 84 us, without 88
-                f32x4_t o[TILES][2], score[3];   // (0, 0), (0, 1), (1, 1)
+                f32x4_t o[HEADS][TILES][2], score[HEADS][3];   // (0, 0), (0, 1), (1, 1)
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
-                    bf16x8_t q[2], kk[2];
+                    bf16x8_t q[HEADS][2], kk[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        u32x4_t f = *reinterpret_cast<const u32x4_t*>(qi + u * 16 * P * 16 + (frag ^ (k * 64)));
-                        if (k == STEPS - 1 && k * 4 + g >= dc) f = u32x4_t{0, 0, 0, 0};   // past head_dim
-                        q[u] = __builtin_bit_cast(bf16x8_t, f);
+#pragma unroll
+                        for (int h = 0; h < HEADS; ++h) {
+                            u32x4_t f = *reinterpret_cast<const u32x4_t*>(qi + (h * 32 + u * 16) * P * 16 + (frag ^ (k * 64)));
+                            if (k == STEPS - 1 && k * 4 + g >= dc) f = u32x4_t{0, 0, 0, 0};   // past head_dim
+                            q[h][u] = __builtin_bit_cast(bf16x8_t, f);
+                        }
                         kk[u] = *reinterpret_cast<const bf16x8_t*>(ki + u * 16 * P * 16 + (frag ^ (k * 64)));
                     }
                     if (k + 1 == STEPS) read_first();
-                    score[0] = product(kk[0], q[0], k == 0 ? zero : score[0]);
-                    score[1] = product(kk[0], q[1], k == 0 ? zero : score[1]);
-                    score[2] = product(kk[1], q[1], k == 0 ? zero : score[2]);
+#pragma unroll
+                    for (int h = 0; h < HEADS; ++h) {
+                        score[h][0] = product(kk[0], q[h][0], k == 0 ? zero : score[h][0]);
+                        score[h][1] = product(kk[0], q[h][1], k == 0 ? zero : score[h][1]);
+                        score[h][2] = product(kk[1], q[h][1], k == 0 ? zero : score[h][2]);
+                    }
 #pragma unroll
                     for (int x = 0; x < TILES; ++x) {
                         f32x4_t lo = s[2 * k][x], hi = s[2 * k + 1][x];
@@ -383,45 +393,52 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
                         const bf16x8_t one = pair(l1, h1);
                         const bf16x8_t two = pair(u32x2_t{f2bf2(lo[0], lo[1]), f2bf2(lo[2], lo[3])}, u32x2_t{f2bf2(hi[0], hi[1]), f2bf2(hi[2], hi[3])});
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) o[x][u] = product(one, q[u], k == 0 ? zero : o[x][u]);
+                        for (int h = 0; h < HEADS; ++h)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) o[x][u] = product(two, q[u], o[x][u]);
+                            for (int u = 0; u < 2; ++u) o[h][x][u] = product(one, q[h][u], k == 0 ? zero : o[h][x][u]);
+#pragma unroll
+                        for (int h = 0; h < HEADS; ++h)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) o[h][x][u] = product(two, q[h][u], o[h][x][u]);
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const float by = since[u] * faded;
+                for (int h = 0; h < HEADS; ++h) {
 #pragma unroll
-                    for (int x = 0; x < TILES; ++x)
+                    for (int u = 0; u < 2; ++u) {
+                        const float by = since[u] * faded;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) o[x][u][r] *= by;
-                }
-                // the chunk's own
+                        for (int x = 0; x < TILES; ++x)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    score[0][r] *= own[r];
-                    score[1][r] *= before[r];
-                    score[2][r] *= own[r];
-                }
+                            for (int r = 0; r < 4; ++r) o[h][x][u][r] *= by;
+                    }
+                    // the chunk's own
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    f32x4_t lo = score[u], hi = u == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : score[2];
-                    const u32x2_t l1 = take_bf16(lo), h1 = take_bf16(hi);
-                    const bf16x8_t one = pair(l1, h1);
-                    const bf16x8_t two = pair(u32x2_t{f2bf2(lo[0], lo[1]), f2bf2(lo[2], lo[3])}, u32x2_t{f2bf2(hi[0], hi[1]), f2bf2(hi[2], hi[3])});
+                    for (int r = 0; r < 4; ++r) {
+                        score[h][0][r] *= own[r];
+                        score[h][1][r] *= before[r];
+                        score[h][2][r] *= own[r];
+                    }
 #pragma unroll
-                    for (int x = 0; x < TILES; ++x) {
-                        o[x][u] = product(v[x], one, o[x][u]);
-                        o[x][u] = product(v[x], two, o[x][u]);
-                        done[u][2 * x] = f2bf2(o[x][u][0], o[x][u][1]);
-                        done[u][2 * x + 1] = f2bf2(o[x][u][2], o[x][u][3]);
+                    for (int u = 0; u < 2; ++u) {
+                        f32x4_t lo = score[h][u], hi = u == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : score[h][2];
+                        const u32x2_t l1 = take_bf16(lo), h1 = take_bf16(hi);
+                        const bf16x8_t one = pair(l1, h1);
+                        const bf16x8_t two = pair(u32x2_t{f2bf2(lo[0], lo[1]), f2bf2(lo[2], lo[3])}, u32x2_t{f2bf2(hi[0], hi[1]), f2bf2(hi[2], hi[3])});
+#pragma unroll
+                        for (int x = 0; x < TILES; ++x) {
+                            o[h][x][u] = product(v[x], one, o[h][x][u]);
+                            o[h][x][u] = product(v[x], two, o[h][x][u]);
+                            done[h][u][2 * x] = f2bf2(o[h][x][u][0], o[h][x][u][1]);
+                            done[h][u][2 * x + 1] = f2bf2(o[h][x][u][2], o[h][x][u][3]);
+                        }
                     }
                 }
             } else {
                 read_first();
             }
             __builtin_amdgcn_s_setprio(0);
-            if (j + 2 < chunks) load(j + 2);
+            if (j + kStages - 1 < chunks) load(j + kStages - 1);
             // the state behind the chunk
             float more;   // by which what is added here counts in the accumulators
             if (OUT) {
@@ -486,7 +503,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
         if (OUT && chunks > 0 && active) store(chunks - 1, count - (chunks - 1) * kChunk);
         float* end = nullptr;
         if (!OUT) end = a.states + (bk * (1 + segments) + segment + 1) * a.D * a.E;
-        else if (a.state_out && segment == last_segment && member == a.group - 1) end = a.state_out + bk * a.D * a.E;
+        else if (a.state_out && segment == last_segment && member + HEADS == a.group) end = a.state_out + bk * a.D * a.E;
         if (end) {
             const Fade fade(age * log_decay);
             int here = lane;   // computed anew: the offsets of the first state's values would stay in registers through the loop
@@ -506,9 +523,11 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
             const int pieces = a.E / 4;
             for (int i = threadIdx.x; i < (rows - behind) * pieces; i += WAVES * 64) {
                 const int64_t row = row0 + behind + i / pieces;
-                *reinterpret_cast<uint2*>(a.out + row * a.ld_o + static_cast<int64_t>(head) * a.E + i % pieces * 4) = make_uint2(0, 0);
+#pragma unroll
+                for (int h = 0; h < HEADS; ++h)
+                    *reinterpret_cast<uint2*>(a.out + row * a.ld_o + static_cast<int64_t>(head + h) * a.E + i % pieces * 4) = make_uint2(0, 0);
             }
-            if (turn_of + 1 < a.heads_each) {   // the next head's loads reuse the stages
+            if (turn_of + 1 < a.turns) {   // the next heads' loads reuse the stages
                 asm volatile("" ::: "memory");
                 s_waitcnt<0, 0>();
                 __builtin_amdgcn_s_barrier();
@@ -559,68 +578,74 @@ int device_cus() {
 }
 
 // How a call runs: token after token for one or two (one token of 16 sequences, 32 heads of 128: 14.8 us against 19.0 for a chunk,
-// two 18.3 against 18.8, four 24.8 against 18.7), else chunks, each sequence in `segments`. The estimates, in us, were checked on
-// 26 shapes on one MI355X (1 to 256 heads of 32 to 128 columns, 256 to 65536 tokens), each in 1 to 256 segments: what they choose
-// is within 7% of the fastest measured on 25, and 10% above it on 4 x 1024 tokens of 32 heads of 128 (73 whole, 67 in 2). A chunk takes a workgroup `step` alone on a CU, and
-// beside others the CU `share` of that for each; a call no less than its bytes at 4.6 TB/s; the first launch 0.55 of a step
-// a chunk; a state's load or store 30 us a MB for a workgroup, and the launch between its states at 2.6 TB/s and 0.08
-// a piece. 4 x 2048 tokens of 32 heads of 128 whole 137 us, in 4 segments 107, in 16 208; one head of 128 with 8192 tokens
-// whole 523, in 64 segments 37, in 256 62; 2 x 300 tokens of 64 heads of 64 whole 16.5, in 2 segments 23.
+// two 18.3 against 18.8, four 24.8 against 18.7), else chunks, each sequence in `segments`, for one query head or two at once.
+// The estimates, in us, were fitted to 70 shapes on one MI355X (1 to 200 heads of 32 to 128 columns, 64 to 65536 tokens), each
+// with one and two heads at once in 1 to 256 segments: what they choose is within 5% of the fastest measured on 61, and
+// 12% above it at worst (5 x 3000 tokens of 32 / 8 heads of 128). A chunk takes a workgroup `step` alone on a CU (two heads 1.45
+// times that), and beside others the CU `share` of it for each; a call no less than its bytes at 4.6 TB/s; the first launch 0.4
+// of a step a chunk; a state's load or store 34 us a MB for a workgroup, and the launch between its states at 4.6 TB/s and 0.09 a
+// piece. 4 x 2048 tokens of 32 heads of 128 whole 137 us, in 4 segments 107, in 16 208; one head of 128 with 8192 tokens
+// whole 523, in 64 segments 37, in 256 62. Two heads at once share the state's update and its splitting, and leave half the
+// workgroups: 32 x 300 tokens of 32 / 8 heads of 128 64 us against 87, 65536 tokens 409 against 526, but 2 x 300 of 64 / 8 heads of
+// 64 19.6 against 16.3.
 struct Plan {
     bool tokens;                    // k_linear_tokens
     int segments, pieces, length;   // as in LinearArgs
+    int heads = 1;                  // of a group, that a workgroup takes at once
 };
 Plan plan(const LinearShape& sh, bool may_split, int64_t cus) {
     if (sh.seq_len <= 2) return Plan{true, 1, 1, static_cast<int>(sh.seq_len)};
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-    const int64_t chunks = up(sh.seq_len, kChunk), heads = sh.batch * sh.heads, rows = sh.batch * sh.kv_heads;
+    const int64_t chunks = up(sh.seq_len, kChunk), rows = sh.batch * sh.kv_heads, group = sh.heads / sh.kv_heads;
     // columns as the kernels compute them
     const double width = static_cast<double>(up(sh.head_dim, 32) * 32 + (sh.value_dim > 64 ? 128 : 64));
-    const double step = 0.1 + 0.0078 * width, share = width >= 192 ? 0.8 : 0.5, alone = sh.value_dim > 64 ? 0.9 : 1.0;
+    const double step = 0.1 + 0.0071 * width, shares[] = {width >= 192 ? 0.82 : 0.73, width >= 192 ? 0.86 : 0.84};
     const double state = 4e-6 * static_cast<double>(sh.head_dim * sh.value_dim);   // MB
-    const double bytes = 2.0 * static_cast<double>(sh.seq_len * (heads + rows) * (sh.head_dim + sh.value_dim));
+    const double bytes = 2.0 * static_cast<double>(sh.seq_len * rows * (group + 1) * (sh.head_dim + sh.value_dim));
     Plan best{false, 1, 1, static_cast<int>(chunks * kChunk)};
     double least = 1e30;
-    for (int64_t want = 1; want == 1 || (may_split && want <= 512 && 2 * want <= chunks); want *= 2)
-        for (int64_t pieces = 1; pieces <= (want > 1 ? 2 : 1); ++pieces) {
-            const int64_t each = up(up(chunks, want), pieces) * pieces, segments = up(chunks, each);
-            const double groups = static_cast<double>(heads * segments), c = static_cast<double>(cus);
-            const double per = step * (groups <= c ? alone : std::max(1.0, share * std::ceil(groups / c)));
-            double cost = 5 + std::max(each * per + std::max(1.0, groups / c) * state * 30, bytes / 4.6e6);
-            if (segments > 1) {
-                const double first = static_cast<double>(rows * (segments - 1) * pieces), all = static_cast<double>(segments * pieces);
-                cost += 3 + each / pieces * 0.55 * step * std::max(1.0, share * std::ceil(first / c)) + std::max(1.0, first / c) * state * 30;
-                cost += 3.5 + 0.08 * all + static_cast<double>(rows) * (all + segments) * state / 2.6;
+    for (int heads = 1; heads <= (group % 2 == 0 ? 2 : 1); ++heads)
+        for (int64_t want = 1; want == 1 || (may_split && want <= 512 && 2 * want <= chunks); want *= 2)
+            for (int64_t pieces = 1; pieces <= (want > 1 ? 2 : 1); ++pieces) {
+                const int64_t each = up(up(chunks, want), pieces) * pieces, segments = up(chunks, each);
+                const double groups = static_cast<double>(rows * (group / heads) * segments), c = static_cast<double>(cus);
+                const double per = step * (heads == 2 ? 1.45 : 1.0) * std::max(1.0, shares[heads - 1] * std::ceil(groups / c));
+                double cost = 5 + std::max(each * per + std::max(1.0, groups / c) * state * 34, bytes / 4.6e6);
+                if (segments > 1) {
+                    const double first = static_cast<double>(rows * (segments - 1) * pieces), all = static_cast<double>(segments * pieces);
+                    cost += 3 + each / pieces * 0.4 * step * std::max(1.0, shares[0] * std::ceil(first / c)) + std::max(1.0, first / c) * state * 34;
+                    cost += 3 + 0.09 * all + static_cast<double>(rows) * (all + segments) * state / 4.6;
+                }
+                if (cost < least) {
+                    least = cost;
+                    best = Plan{false, static_cast<int>(segments), static_cast<int>(pieces), static_cast<int>(each / pieces * kChunk), heads};
+                }
             }
-            if (cost < least) {
-                least = cost;
-                best = Plan{false, static_cast<int>(segments), static_cast<int>(pieces), static_cast<int>(each / pieces * kChunk)};
-            }
-        }
     return best;
 }
 
-template <int STEPS, int TILES, int WAVES, bool OUT>
+template <int STEPS, int TILES, int WAVES, int HEADS>
 void launch(const LinearArgs& a, int64_t groups, hipStream_t s) {
-    k_linear_chunks<STEPS, TILES, WAVES, OUT><<<grid_of(groups, WAVES * 64), WAVES * 64, 0, s>>>(a);
+    k_linear_chunks<STEPS, TILES, WAVES, HEADS><<<grid_of(groups, WAVES * 64), WAVES * 64, 0, s>>>(a);
     launch_check("attention_linear");
 }
 // More than 64 value columns to four waves of 32, or where a workgroup has its CU to itself to eight of 16, which take a chunk in
-// 0.9 of the time (8 heads of 128 with 100 tokens 16.3 us against 18.0) and two workgroups' chunks in 1.2 of it.
-template <int STEPS, bool OUT>
+// 0.9 of the time (8 heads of 128 with 100 tokens 16.3 us against 18.0; two heads at once in 0.94 to 1.02) and two workgroups' chunks
+// in 1.2 of it.
+template <int STEPS, int HEADS>
 void by_values(const LinearArgs& a, int64_t groups, int64_t cus, hipStream_t s) {
-    if (a.E <= 64) return launch<STEPS, 1, 4, OUT>(a, groups, s);
-    if constexpr (OUT)
-        if (groups <= cus) return launch<STEPS, 1, 8, OUT>(a, groups, s);
-    launch<STEPS, 2, 4, OUT>(a, groups, s);
+    if (a.E <= 64) return launch<STEPS, 1, 4, HEADS>(a, groups, s);
+    if constexpr (HEADS > 0)
+        if (groups <= cus) return launch<STEPS, 1, 8, HEADS>(a, groups, s);
+    launch<STEPS, 2, 4, HEADS>(a, groups, s);
 }
-template <bool OUT>
+template <int HEADS>
 void by_width(const LinearArgs& a, int64_t groups, int64_t cus, hipStream_t s) {
     switch ((a.D + 31) / 32) {
-        case 1: return by_values<1, OUT>(a, groups, cus, s);
-        case 2: return by_values<2, OUT>(a, groups, cus, s);
-        case 3: return by_values<3, OUT>(a, groups, cus, s);
-        default: return by_values<4, OUT>(a, groups, cus, s);
+        case 1: return by_values<1, HEADS>(a, groups, cus, s);
+        case 2: return by_values<2, HEADS>(a, groups, cus, s);
+        case 3: return by_values<3, HEADS>(a, groups, cus, s);
+        default: return by_values<4, HEADS>(a, groups, cus, s);
     }
 }
 
@@ -636,7 +661,7 @@ int64_t attention_linear_workspace_floats(const LinearShape& sh) {
 bh_attention_linear_plan attention_linear_plan(const LinearShape& sh, bool may_split, int cus) {
     const Plan how = plan(sh, may_split, cus > 0 ? cus : device_cus());
     if (how.tokens) return bh_attention_linear_plan{1, 1, sh.batch * sh.kv_heads * ((sh.value_dim + 31) / 32)};
-    return bh_attention_linear_plan{kChunk, how.segments, sh.batch * sh.heads * how.segments};
+    return bh_attention_linear_plan{kChunk, how.segments, sh.batch * sh.heads / how.heads * how.segments};
 }
 
 void launch_attention_linear(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16_t* out, const LinearShape& sh,
@@ -669,15 +694,16 @@ void launch_attention_linear(const bf16_t* q, const bf16_t* k, const bf16_t* v, 
     const bool in_place = state_in && state_in == state_out && a.group > 1;
     const bool copied = how.segments > 1 || (in_place && ws);
     a.first_state = copied ? 2 : state_in ? 1 : 0;
-    a.heads_each = in_place && !copied ? a.group : 1;
-    const int64_t groups = rows * how.segments * (a.group / a.heads_each);
+    a.turns = in_place && !copied ? a.group / how.heads : 1;
+    const int64_t groups = rows * how.segments * (a.group / how.heads / a.turns);
     require(groups < (int64_t{1} << 31) && rows * how.segments * how.pieces < (int64_t{1} << 31), "attention_linear: too many heads");
-    if (how.segments > 1) by_width<false>(a, rows * (how.segments - 1) * how.pieces, cus, s);
+    if (how.segments > 1) by_width<0>(a, rows * (how.segments - 1) * how.pieces, cus, s);
     if (copied) {
         k_linear_carry<<<grid_of((rows * a.D * a.E / 4 + kThreads - 1) / kThreads, kThreads), kThreads, 0, s>>>(a);
         launch_check("attention_linear");
     }
-    by_width<true>(a, groups, cus, s);
+    if (how.heads == 2) by_width<2>(a, groups, cus, s);
+    else by_width<1>(a, groups, cus, s);
 }
 
 }  // namespace bh

@@ -434,3 +434,62 @@ def test_a_block_of_linear_attention(hip):
     for got, want in ((one_stream, stream[:, n - 1:]), (one_after, after[:, n - 1:])):
         assert (got.float() - want.float()).abs().max() <= 4 * 2.0 ** -8 * want.float().abs().max()
     assert (one_state - state).abs().max() <= 2.0 ** -8 * state.abs().max()
+
+
+def heads_at_once(batch, heads, kvh, n, d, e, with_workspace=True):
+    plan = bh.AttentionLinearPlan()
+    bh.call("bh_attention_linear_describe", batch, heads, kvh, n, d, e, int(with_workspace), 0, ctypes.byref(plan))
+    return batch * heads * plan.segments / plan.workgroups
+
+
+# enough workgroups that two heads of a group share one, with a CU to themselves or not; 65 tokens end in a chunk of one
+@pytest.mark.parametrize("d", [8, 24, 32, 40, 64, 72, 96, 104, 128])
+@pytest.mark.parametrize("batch,heads,kvh", [(8, 64, 16), (24, 48, 8)])
+def test_two_heads_at_once(hip, batch, heads, kvh, d):
+    for n, e in ((65, d), (20, 136 - d if d < 128 else 8)):
+        assert heads_at_once(batch, heads, kvh, n, d, e) == 2
+        check(batch, heads, kvh, n, d, e, lens=[max(0, n - 9 * (b % 9)) for b in range(batch)], seed=d)
+
+
+@pytest.mark.parametrize("n,batch,heads,kvh,d", [(50, 12, 64, 16, 128), (50, 12, 32, 16, 128), (3000, 2, 16, 4, 128), (3000, 4, 12, 2, 64)])
+def test_two_heads_at_once_in_place_and_captured(hip, n, batch, heads, kvh, d):
+    """The state in place, with a workspace and without, where a workgroup takes a group's heads in turns of two; a replay."""
+    import torch
+    q, k, v = inputs(batch, heads, kvh, n, d, d, n)
+    state, rate = normal((batch, kvh, d, d), 9, 1.0, torch.float32), decays(kvh)
+    want, tol, new_want, new_tol = plain(q, k, v, rate, None, state)
+    for with_workspace in (True, False):
+        if with_workspace:
+            assert heads_at_once(batch, heads, kvh, n, d, d) == 2
+        out, new = run(q, k, v, rate, None, state, with_workspace=with_workspace, in_place=True)
+        compare(out, want, tol)
+        compare(new, new_want, new_tol, "state")
+    (ws, need), out, new = workspace(q, k, v), torch.zeros_like(v.new_empty(batch, n, heads, d)), torch.zeros_like(state)
+    eager = run(q, k, v, rate, None, state)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(q, k, v, out, rate, None, state, new, 0.0, ws, need, torch.cuda.current_stream())
+    for _ in range(3):
+        out.fill_(3.0)
+        new.fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager[0]) and torch.equal(new, eager[1])
+
+
+@pytest.mark.parametrize("poison", [math.nan, math.inf])
+def test_a_head_of_two_at_once_stays_alone(hip, poison):
+    """What is wrong with one query head's queries does not reach the head beside it, the other groups or the state."""
+    import torch
+    batch, heads, kvh, n, d = 12, 64, 16, 50, 64
+    assert heads_at_once(batch, heads, kvh, n, d, d) == 2
+    q, k, v = inputs(batch, heads, kvh, n, d, d, 3)
+    rate = decays(kvh)
+    clean, state = run(q, k, v, rate)
+    q[:, 17, 6] = poison
+    out, new = run(q, k, v, rate)
+    others = [h for h in range(heads) if h != 6]
+    assert torch.equal(out[:, :, others], clean[:, :, others]) and torch.equal(new, state)
+    assert not out[:, 17, 6].isfinite().any()
+    assert torch.equal(out[:, :17, 6], clean[:, :17, 6]) and torch.equal(out[:, 18:, 6], clean[:, 18:, 6])

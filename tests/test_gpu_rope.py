@@ -220,3 +220,18 @@ def test_in_a_graph_and_on_two_streams(hip):
         graph.replay()
         torch.cuda.synchronize()
         compare(outs[0], x, p, bh.RopeAxes.of([16, 16], interleaved=True))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_keys_alone(hip, dtype):
+    """No query heads, as for the keys of another sequence: q and q_out may be NULL."""
+    import torch
+    t, code = dtypes()[dtype]
+    axes = bh.RopeAxes.of([8, 12, 12], interleaved=True)
+    positions = grid(77, 3, 1)
+    k = normal((231, 5, 64), 2, t)
+    out = torch.full_like(k, 7.0)
+    bh.call("bh_rope", ctypes.byref(axes), positions.data_ptr(), 77, None, 0, None, 0, 0, k.data_ptr(), 320, out.data_ptr(), 320, 5, 231, 64,
+            0, code, bh.stream_ptr(None))
+    torch.cuda.synchronize()
+    compare(out, k, positions, axes)
