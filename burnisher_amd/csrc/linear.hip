@@ -20,8 +20,9 @@
 // What bounds it: one token of 16 sequences, 32 states of 128 x 128 each, their bytes (14.9 us, 4.5 TB/s). Chunks, the
 // instructions of few waves: at 128 x 128 a chunk takes 2.3 us alone on a CU, two 3.9, where matrix (100, 1600 cycles) and vector
 // instructions (361) of two waves of a SIMD overlap little, and issuing a wave's six direct loads takes 500 to 800 cycles of 6500.
-// 2 x 4096 tokens of 32 / 8 heads of 128 83 us, 65 of it the third launch; 65536 tokens of 16 heads of 128 356 us, near its
-// bytes: k and v twice, 108 us of it the first launch (4.8 TB/s), 15 the second; 2 x 300 of 64 heads of 64 16.6 us.
+// Two heads at once take 152 and 430 instead of 200 and 722: 2 x 4096 tokens of 32 / 8 heads of 128 71 us (83 with one), 51 of
+// it the third launch; 65536 tokens of 16 heads of 128 351 us, near its bytes: k and v twice, 106 us of it the first launch
+// (4.9 TB/s), 15 the second; 2 x 300 of 64 heads of 64 16.8 us.
 #include "common.h"
 
 #include <algorithm>
@@ -364,7 +365,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
             if constexpr (OUT) {
                 // by 32 rows of the state: scores of key tile y against query tile u >= y, and the state's part of the outputs
                 const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-                __builtin_amdgcn_s_setprio(1);   // before the other wave's loads and values: 2 x 4096 tokens of 32 / 8 heads of 128 84 us, without 88
+                __builtin_amdgcn_s_setprio(1);   // before the other wave's loads and values: 2 x 4096 tokens of 32 / 8 heads of 128, one at once, 84 us, without 88
                 f32x4_t o[HEADS][TILES][2], score[HEADS][3];   // (0, 0), (0, 1), (1, 1)
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
