@@ -520,14 +520,14 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
                     }
         }
         if (OUT) {   // the outputs behind the sequence
+            // by rows: a count of 8-byte pieces passes 2^31 from 2^26 rows of 128 columns on
             const int behind = max(n - first, 0), rows = min(a.N - first, length);
-            const int pieces = a.E / 4;
-            for (int i = threadIdx.x; i < (rows - behind) * pieces; i += WAVES * 64) {
-                const int64_t row = row0 + behind + i / pieces;
+            const int pieces = a.E / 4, each = WAVES * 64 / pieces, piece = threadIdx.x % pieces;
+            if (static_cast<int>(threadIdx.x) < each * pieces)
+                for (int i = behind + threadIdx.x / pieces; i < rows; i += each)
 #pragma unroll
-                for (int h = 0; h < HEADS; ++h)
-                    *reinterpret_cast<uint2*>(a.out + row * a.ld_o + static_cast<int64_t>(head + h) * a.E + i % pieces * 4) = make_uint2(0, 0);
-            }
+                    for (int h = 0; h < HEADS; ++h)
+                        *reinterpret_cast<uint2*>(a.out + (row0 + i) * a.ld_o + static_cast<int64_t>(head + h) * a.E + piece * 4) = make_uint2(0, 0);
             if (turn_of + 1 < a.turns) {   // the next heads' loads reuse the stages
                 asm volatile("" ::: "memory");
                 s_waitcnt<0, 0>();

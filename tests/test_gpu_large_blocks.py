@@ -61,3 +61,29 @@ def test_norms_of_many_rows(hip):
     for g, w in zip(got, want):
         assert (g[-64:] == 9.0).all(), "written past the end"
         assert (g[:-64].view(times, piece * cols) == w.view(-1)).all()
+
+
+# 2^26 tokens of 32 8-byte pieces: from there on a count of pieces behind the sequence passes 31 bits
+@pytest.mark.parametrize("n", [2 ** 26, 2 ** 26 + 1, 2 ** 26 + 32])
+def test_linear_attention_of_a_token_before_long_padding(hip, n):
+    import torch
+    d, e = 8, 128
+    plan = bh.AttentionLinearPlan()
+    bh.call("bh_attention_linear_describe", 1, 1, 1, n, d, e, 0, 0, ctypes.byref(plan))
+    assert (plan.chunk, plan.segments) == (32, 1)
+    rate, lens = decays(1), torch.tensor([1], dtype=torch.int32, device="cuda")
+    first = [normal((1, 40, 1, w), s) for s, w in ((1, d), (2, d), (3, e))]
+    want, new, new_want = torch.zeros(1, 40, 1, e, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 1, d, e, device="cuda"), torch.zeros(1, 1, d, e, device="cuda")
+    call(*first, want, rate, lens, None, new_want, 0.0, None, 0)
+    long = [torch.empty(1, n, 1, w, dtype=torch.bfloat16, device="cuda") for w in (d, d, e)]
+    for t, x in zip(long, first):
+        t[:, :1] = x[:, :1]
+    # 4096 bytes before and behind the output stay as they are
+    buffer = torch.full((n * e + 4096,), 9.0, dtype=torch.bfloat16, device="cuda")
+    out = buffer[2048:-2048].view(1, n, 1, e)
+    call(*long, out, rate, lens, None, new, 0.0, None, 0)
+    torch.cuda.synchronize()
+    assert want[0, 0].any() and torch.equal(out[0, 0], want[0, 0]) and torch.equal(new, new_want)
+    for i in range(1, n, 2 ** 22):
+        assert not out[0, i:i + 2 ** 22].any(), f"rows from {i} on are not zeros"
+    assert (buffer[:2048] == 9.0).all() and (buffer[-2048:] == 9.0).all()
