@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int d = t / 2 * 32 + (here >> 4) * 8 + t % 2 * 4 + r, e = column_of(x, here & 15);
-                        if (d < a.D && e < a.E) end[d * a.E + e] = fade(s[t][x][r]);
+                        if (d < a.D && e < a.E) end[d * a.E + e] = age > 0 ? fade(s[t][x][r]) : s[t][x][r];   // of no tokens as it is, infinities too
                     }
         }
         if (OUT) {   // the outputs behind the sequence

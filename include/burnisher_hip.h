@@ -317,7 +317,9 @@ int bh_rope(const bh_rope_axes* axes, const int32_t* positions, int64_t position
  * product they are sums of two or three bf16 terms (16 bits and more of a score or state that enters an
  * output, 24 of what enters a state), so a bf16 output is off by its own rounding and little else. An infinity or NaN
  * in a key or value reaches the outputs and the state behind it for as long as its weight is not zero in fp32
- * (and may for longer), and may reach the outputs of the 31 tokens before it. Element (b, s, h, d) of q lives at
+ * (and may for longer), and may reach the outputs of the 31 tokens before it. One in state_in is handed on as it is where a
+ * sequence has no tokens; behind a token an infinity may have become a NaN. A value, a score q . k, a state or a q . S above
+ * 2^119 may overflow on its way. Element (b, s, h, d) of q lives at
  * q[(b * seq_len + s) * ld_q + h * head_dim + d], likewise k, and v and out with value_dim. head_dim and
  * value_dim are multiples of 8 up to 128, the row strides multiples of 8 (ld_out of 4) and ld_q, ld_k and
  * ld_v below 2^24, q, k and v 16-byte, out 8-byte and the states 16-byte aligned, seq_len below 2^30 and
