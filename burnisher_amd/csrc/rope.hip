@@ -149,6 +149,8 @@ void launch_rope(const bh_rope_axes& axes, const int32_t* positions, int64_t pos
             const int m = first + j;
             if (j == 0 || m % 8 == 0) high = power(m / 8 * 8, n);
             a.turns[i] = axes.scale[x] * (high * low[m % 8]) / (2.0 * M_PI);
+            // else a position times it, or nothing times it, is a NaN
+            require(std::isfinite(a.turns[i] * 0x1p31), "rope: a position times scale and frequency leaves the range of fp64");
             a.axis[i] = static_cast<uint8_t>(x);
         }
     }

@@ -280,7 +280,8 @@ int bh_attention_window_describe(int64_t batch, int64_t heads, int64_t kv_heads,
  * width of a video). Each axis turns pairs of columns of a head: pair i, columns (u, v), becomes
  *   (u cos t - v sin t, u sin t + v cos t),  t = position on the pair's axis * scale[axis] * frequency.
  * The pairs are numbered axis by axis, pairs[0] of the first axis first. The angles are computed in fp64
- * and reduced to one turn before their sine and cosine are taken in fp32, so far positions keep theirs. */
+ * and reduced to one turn before their sine and cosine are taken in fp32, so far positions keep theirs; axes
+ * whose scale times frequency times 2^31 is not finite in fp64 are refused. */
 typedef struct bh_rope_axes {
     int axes;            /* 1 to 4 */
     int pairs[4];        /* pairs of columns that each axis turns; at most 128 in all */

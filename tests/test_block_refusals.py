@@ -52,6 +52,14 @@ def test_rope_refuses_axes(over, says):
     assert says in rope(axes_with(**over))
 
 
+# scale times frequency, or that times the farthest position, is no finite number in 64 bits
+@pytest.mark.parametrize("over", [
+    dict(theta=1e-300, scale=[1e100, 1.0, 1.0, 1.0]), dict(theta=1e-300, scale=[1.0, 1e100, 1.0, 1.0]), dict(scale=[1.0, 1.5e300, 1.0, 1.0]),
+    dict(scale=[-1.7e308, 1.0, 1.0, 1.0]), dict(theta=5e-324, scale=[1.0, 1e60, 1.0, 1.0], joint=1)])
+def test_rope_refuses_angles_without_a_value(over):
+    assert "range of fp64" in rope(axes_with(**over))
+
+
 def test_rope_refuses_no_axes():
     assert "axes is null" in rope(False)
     for pairs, scale in (([], ()), ([1] * 5, ()), ([1], (1.0, 1.0))):
