@@ -634,6 +634,11 @@ int bh_attention_linear(const void* q, int64_t ld_q, const void* k, int64_t ld_k
                 "attention_linear: q, k and v must be 16-byte, out 8-byte aligned");
         require(aligned(state_in, 16) && aligned(state_out, 16), "attention_linear: a state is not 16-byte aligned");
         require(aligned(log_decay, 4) && aligned(lens, 4), "attention_linear: an operand is not aligned to its type");
+        if (seq_len > 0) {   // a workgroup would write what another one has still to read
+            require(out != q, "attention_linear: out is q");
+            require(out != k, "attention_linear: out is k");
+            require(out != v, "attention_linear: out is v");
+        }
         sh.ld_q = ld_q;
         sh.ld_k = ld_k;
         sh.ld_v = ld_v;

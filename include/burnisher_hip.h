@@ -309,8 +309,9 @@ int bh_rope(const bh_rope_axes* axes, const int32_t* positions, int64_t position
  *   out_t = scale * q_t . S_t
  * from S before the first token in state_in (NULL: zeros) to S behind the last one in state_out (NULL: not
  * wanted), both fp32 [batch, kv_heads, head_dim, value_dim]; state_out may be state_in and must not overlap
- * it otherwise. One token against a state and a long prompt are the same call: sizes choose between a kernel
- * that takes token after token and one of chunks, whose sequence is split where there are few heads.
+ * it otherwise. out must not overlap q, k or v, but may lie beside them in the rows of one buffer. One token
+ * against a state and a long prompt are the same call: sizes choose between a kernel that takes token after
+ * token and one of chunks, whose sequence is split where there are few heads.
  * `log_decay` is fp32 [kv_heads] on the device; a value above 0, or NaN, counts as 0 (no decay), and -infinity
  * forgets everything but the token itself. `lens` (NULL: seq_len) is int32 [batch] on the device, taken as at
  * least 0 and at most seq_len: a sequence ends there, nothing behind it is read and its outputs are zeros.

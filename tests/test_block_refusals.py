@@ -90,6 +90,12 @@ def test_linear_refuses(over, says):
     assert says in linear(**over)
 
 
+@pytest.mark.parametrize("same", ["q", "k", "v"])
+def test_linear_refuses_an_output_on_an_input(same):
+    apart = {name: D + (i << 20) for i, name in enumerate(("q", "k", "v"))}
+    assert "out is " + same in linear(**apart, out=apart[same], ld_v=576, ld_q=576, ld_k=576)
+
+
 def norms(plan=None, **over):
     a = dict(x=D, ld_x=64, residual=D, ld_res=64, residual_out=D, ld_res_out=64, out=D, ld_out=64, rows=4, cols=64)
     kinds = dict(residual_dtype=bh.BF16, dtype=bh.BF16)
