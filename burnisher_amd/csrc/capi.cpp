@@ -575,6 +575,7 @@ LinearShape linear_shape(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
     require_nonneg(heads, op, "heads");
     require_nonneg(seq_len, op, "seq_len");
     require(kv_heads > 0 && heads % kv_heads == 0, "attention_linear: heads must be a multiple of kv_heads");
+    require(kv_heads < kSizeLimit, "attention_linear: kv_heads must be below 2^30");   // with no heads, a multiple of any number
     require(head_dim > 0 && head_dim <= 128 && head_dim % 8 == 0 && value_dim > 0 && value_dim <= 128 && value_dim % 8 == 0,
             "attention_linear (hip-gfx950): head_dim and value_dim must be multiples of 8 up to 128");
     require(batch < kSizeLimit && heads < kSizeLimit && seq_len < kSizeLimit, "attention_linear: seq_len must be below 2^30");
@@ -619,6 +620,7 @@ int bh_attention_linear(const void* q, int64_t ld_q, const void* k, int64_t ld_k
                 "attention_linear: ld_q, ld_k and ld_v must be multiples of 8, ld_out of 4");
         const int64_t most = int64_t{1} << 24;
         require(ld_q < most && ld_k < most && ld_v < most, "attention_linear: ld_q, ld_k and ld_v must be below 2^24");
+        require(heads > 0 || batch == 0 || !state_out, "attention_linear: state_out without query heads");
         if (batch * heads == 0 || (seq_len == 0 && !state_out)) return;
         if (seq_len > 0) {   // without tokens the state is copied
             require_device_ptr(q, op, "q");

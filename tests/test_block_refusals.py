@@ -96,6 +96,15 @@ def test_linear_refuses_an_output_on_an_input(same):
     assert "out is " + same in linear(**apart, out=apart[same], ld_v=576, ld_q=576, ld_k=576)
 
 
+def test_linear_refuses_a_state_without_query_heads():
+    """Without query heads there is no call to make; one that is asked for a state may not leave it unwritten."""
+    assert "query heads" in linear(heads=0, ld_q=0, ld_o=0, state_out=D)
+    assert "kv_heads must be" in linear(heads=0, ld_q=0, ld_o=0, kvh=1 << 60)
+    lib = bh.lib()
+    assert lib.bh_attention_linear(None, 0, D, 64, D, 64, None, 0, 2, 0, 1, 5, 64, 64, 0.0, None, None, None, None, bh.BF16, None, 0, None) == 0
+    assert lib.bh_attention_linear(None, 0, None, 64, None, 64, None, 0, 0, 0, 1, 5, 64, 64, 0.0, None, None, None, D, bh.BF16, None, 0, None) == 0
+
+
 def norms(plan=None, **over):
     a = dict(x=D, ld_x=64, residual=D, ld_res=64, residual_out=D, ld_res_out=64, out=D, ld_out=64, rows=4, cols=64)
     kinds = dict(residual_dtype=bh.BF16, dtype=bh.BF16)
