@@ -133,6 +133,11 @@ class ResidualNorms(ctypes.Structure):
                 ("shift", ctypes.c_void_p), ("mod_rows", ctypes.c_int64), ("ld_mod", ctypes.c_int64),
                 ("weight_offset", ctypes.c_float)]
 
+    def __init__(self, *args, **fields):
+        """Fields as in C, but the branch and the residual enter with a factor of 1 unless one is given."""
+        self.branch_scale = self.residual_scale = 1.0
+        super().__init__(*args, **fields)
+
 
 class SchedCoefficients(ctypes.Structure):
     _fields_ = [("order", ctypes.c_int)] + [

@@ -361,7 +361,7 @@ typedef struct bh_residual_norms {
     const void* post_bias;
     float post_eps;
     const void* gate;          /* rows of cols elements ld_mod apart, as scale and shift: one per mod_rows rows */
-    float branch_scale, residual_scale;
+    float branch_scale, residual_scale;   /* factors as they are: 0, as in a zeroed struct, drops its term, so set both */
     int pre_norm;
     const void* pre_weight;
     const void* pre_bias;

@@ -158,3 +158,14 @@ def test_empty_calls_are_no_ops():
     assert lib.bh_attention_linear(None, 64, None, 64, None, 64, None, 64, 0, 1, 1, 5, 64, 64, 0.0, None, None, None, None, bh.BF16, None, 0, None) == 0
     assert lib.bh_attention_linear(None, 64, None, 64, None, 64, None, 64, 2, 1, 1, 0, 64, 64, 0.0, None, None, None, None, bh.BF16, None, 0, None) == 0
     assert lib.bh_residual_norms_run(None, 64, None, 64, D, 64, None, 64, 0, 64, ctypes.byref(plan), bh.F32, bh.BF16, None) == 0
+
+
+def test_norms_struct_keeps_what_its_caller_does_not_name():
+    """Factors that are not named are 1, those that are stay as given; a zeroed struct of C has 0."""
+    plan = bh.ResidualNorms()
+    assert (plan.branch_scale, plan.residual_scale) == (1.0, 1.0)
+    assert (plan.post_norm, plan.pre_norm, plan.gate, plan.mod_rows, plan.weight_offset) == (bh.NORM_NONE, bh.NORM_NONE, None, 0, 0.0)
+    plan = bh.ResidualNorms(post_norm=bh.NORM_RMS, branch_scale=0.0, residual_scale=0.5)
+    assert (plan.post_norm, plan.branch_scale, plan.residual_scale) == (bh.NORM_RMS, 0.0, 0.5)
+    plan = bh.ResidualNorms(bh.NORM_LAYER, None, None, 0.25, None, 3.0)
+    assert (plan.post_norm, plan.post_eps, plan.branch_scale, plan.residual_scale) == (bh.NORM_LAYER, 0.25, 3.0, 1.0)
