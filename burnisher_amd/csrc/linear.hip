@@ -655,8 +655,8 @@ void by_width(const LinearArgs& a, int64_t groups, int64_t cus, hipStream_t s) {
 int64_t attention_linear_workspace_floats(const LinearShape& sh) {
     const Plan how = plan(sh, true, device_cus());
     const int64_t states = sh.batch * sh.kv_heads * sh.head_dim * sh.value_dim;
-    // one state each where a group's heads would still read what one of them writes
-    return how.segments > 1 ? (1 + (how.segments - 1) * how.pieces) * states : !how.tokens && sh.heads > sh.kv_heads ? states : 0;
+    // one state each where some of a group's workgroups would still read what one of them writes
+    return how.segments > 1 ? (1 + (how.segments - 1) * how.pieces) * states : !how.tokens && sh.heads / sh.kv_heads > how.heads ? states : 0;
 }
 
 bh_attention_linear_plan attention_linear_plan(const LinearShape& sh, bool may_split, int cus) {
@@ -691,8 +691,8 @@ void launch_attention_linear(const bf16_t* q, const bf16_t* k, const bf16_t* v, 
         launch_check("attention_linear");
         return;
     }
-    // a group's workgroups read the first state while one of them may end and write it in place
-    const bool in_place = state_in && state_in == state_out && a.group > 1;
+    // a group's workgroups, where it has several, read the first state while one of them may end and write it in place
+    const bool in_place = state_in && state_in == state_out && a.group > how.heads;
     const bool copied = how.segments > 1 || (in_place && ws);
     a.first_state = copied ? 2 : state_in ? 1 : 0;
     a.turns = in_place && !copied ? a.group / how.heads : 1;

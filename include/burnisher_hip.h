@@ -326,7 +326,8 @@ int bh_rope(const bh_rope_axes* axes, const int32_t* positions, int64_t position
  * value_dim are multiples of 8 up to 128, the row strides multiples of 8 (ld_out of 4) and ld_q, ld_k and
  * ld_v below 2^24, q, k and v 16-byte, out 8-byte and the states 16-byte aligned, seq_len below 2^30 and
  * batch * heads below 2^31. A call without query heads does nothing, and is refused where it asks for state_out.
- * `workspace` as in bh_gemm_fp8: the states of a split sequence. It has no counterpart in the reference. */
+ * `workspace` as in bh_gemm_fp8: the states of a split sequence, and first states that several workgroups read while
+ * one may write them in place. It has no counterpart in the reference. */
 int bh_attention_linear(const void* q, int64_t ld_q, const void* k, int64_t ld_k, const void* v,
                         int64_t ld_v, void* out, int64_t ld_out, int64_t batch, int64_t heads,
                         int64_t kv_heads, int64_t seq_len, int64_t head_dim, int64_t value_dim,

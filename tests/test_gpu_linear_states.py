@@ -42,3 +42,21 @@ def test_an_empty_sequence_hands_its_state_on(hip, name, with_workspace, in_plac
         out, new = run(q, k, v, rate, lens, state, with_workspace=with_workspace, in_place=in_place)
         assert torch.equal(new[0].view(torch.int32), state[0].view(torch.int32)), tokens
         assert not out[0].any() and out[1:].isfinite().all() and new[1:].isfinite().all()
+
+
+# unsplit chunks: a workgroup with all heads of a key head alone reads and writes its state; others need the first state kept apart
+@pytest.mark.parametrize("batch,heads,kvh,n,d,apart", [(12, 32, 16, 50, 128, False), (16, 32, 32, 100, 64, False), (12, 64, 16, 50, 64, True),
+                                                       (3, 4, 2, 40, 64, True)])
+def test_a_state_is_kept_apart_only_where_heads_share_it(hip, batch, heads, kvh, n, d, apart):
+    import torch
+    plan = bh.AttentionLinearPlan()
+    bh.call("bh_attention_linear_describe", batch, heads, kvh, n, d, d, 1, 0, ctypes.byref(plan))
+    assert (plan.chunk, plan.segments) == (32, 1) and (batch * kvh < plan.workgroups) == apart
+    q, k, v = inputs(batch, heads, kvh, n, d, d, 1)
+    need = bh.lib().bh_attention_linear_workspace_bytes(batch, heads, kvh, n, d, d)
+    assert need == (4 * batch * kvh * d * d if apart else 0)
+    state, rate = normal((batch, kvh, d, d), 2, 1.0, torch.float32), decays(kvh)
+    want = run(q, k, v, rate, None, state)
+    for with_workspace in (True, False):
+        got = run(q, k, v, rate, None, state, with_workspace=with_workspace, in_place=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
