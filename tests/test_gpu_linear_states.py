@@ -60,3 +60,30 @@ def test_a_state_is_kept_apart_only_where_heads_share_it(hip, batch, heads, kvh,
     for with_workspace in (True, False):
         got = run(q, k, v, rate, None, state, with_workspace=with_workspace, in_place=True)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("name", FORMS)
+def test_states_keep_24_bits_in_every_form(hip, name):
+    """One token holds a key, so an element of the state is decay^(n - 1 - t) k v, and what it is off by is counted in units of 2^-24.
+
+    The weight: two exponentials of 2, each with an exponent off by 2.5 of itself, and their product, 5; times the value 1, in three
+    bf16 terms 1, added up one by one 3. In the sequence's last segment, or an unsplit one, the put-off decay 3 where it is applied
+    on the way and 5 behind the last token. A piece of a split adds 1 for each piece behind it, whose decays are
+    all near 1 here, and the other products are zeros. Together 24, the pieces behind, and 6 for each e-fold of the decay. A third
+    term left out would be up to 64."""
+    import torch
+    batch, heads, kvh, n, d = form(name)
+    plan = bh.AttentionLinearPlan()
+    bh.call("bh_attention_linear_describe", batch, heads, kvh, n, d, d, 1, 0, ctypes.byref(plan))
+    rate = torch.linspace(-1e-4, -3e-5, kvh, device="cuda")
+    q, k, v = inputs(batch, heads, kvh, n, d, d, 7)
+    for t in {0, n // 2, max(0, n - 3 * n // (2 * plan.segments)), max(0, n - 40), n - 1}:
+        one = torch.zeros_like(k)
+        one[:, t] = k[:, t]
+        out, new = run(q, one, v, rate)
+        fade = rate.double() * (n - 1 - t)
+        want = torch.exp(fade)[None, :, None, None] * k[:, t].double()[..., :, None] * v[:, t].double()[..., None, :]
+        pieces = 0 if plan.segments == 1 else 2 * ((n - t) * plan.segments // n + 1)
+        slack = 2.0 ** -24 * (24 + pieces + 6 * fade.abs()[None, :, None, None])
+        assert ((new.double() - want).abs() <= want.abs() * slack + 1e-37).all(), t
+        assert not out[:, :t].any()
