@@ -506,7 +506,15 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
         if (!OUT) end = a.states + (bk * (1 + segments) + segment + 1) * a.D * a.E;
         else if (a.state_out && segment == last_segment && member + HEADS == a.group) end = a.state_out + bk * a.D * a.E;
         if (end) {
-            const Fade fade(age * log_decay);
+            if (age > 0) {   // of no tokens as it is, infinities too
+                const Fade fade(age * log_decay);
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int x = 0; x < TILES; ++x)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[t][x][r] = fade(s[t][x][r]);
+            }
             int here = lane;   // computed anew: the offsets of the first state's values would stay in registers through the loop
             asm volatile("" : "+v"(here));
 #pragma unroll
@@ -516,7 +524,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_linear_chunks(LinearArgs a) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int d = t / 2 * 32 + (here >> 4) * 8 + t % 2 * 4 + r, e = column_of(x, here & 15);
-                        if (d < a.D && e < a.E) end[d * a.E + e] = age > 0 ? fade(s[t][x][r]) : s[t][x][r];   // of no tokens as it is, infinities too
+                        if (d < a.D && e < a.E) end[d * a.E + e] = s[t][x][r];
                     }
         }
         if (OUT) {   // the outputs behind the sequence

@@ -70,7 +70,7 @@ def test_states_keep_24_bits_in_every_form(hip, name):
     bf16 terms 1, added up one by one 3. In the sequence's last segment, or an unsplit one, the put-off decay 3 where it is applied
     on the way and 5 behind the last token. A piece of a split adds 1 for each piece behind it, whose decays are
     all near 1 here, and the other products are zeros. Together 24, the pieces behind, and 6 for each e-fold of the decay. A third
-    term left out would be up to 64."""
+    term left out would be up to 256 (half a bf16 step of half a step)."""
     import torch
     batch, heads, kvh, n, d = form(name)
     plan = bh.AttentionLinearPlan()
