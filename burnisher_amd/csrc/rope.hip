@@ -141,6 +141,7 @@ void launch_rope(const bh_rope_axes& axes, const int32_t* positions, int64_t pos
     for (int x = 0; x < axes.axes; ++x) a.pairs += axes.pairs[x];
     // theta^(-m / n) = theta^(-8 (m / 8) / n) theta^(-(m % 8) / n): 16 powers for 64 pairs, whose 64 would take longer than the launch
     auto power = [&](int m, int n) { return std::pow(axes.theta, -static_cast<double>(m) / n); };
+    bool finite = true;
     for (int x = 0, i = 0; x < axes.axes; ++x) {
         const int n = axes.joint ? a.pairs : axes.pairs[x], first = axes.joint ? i : 0;
         double low[8], high = 0.0;
@@ -149,11 +150,11 @@ void launch_rope(const bh_rope_axes& axes, const int32_t* positions, int64_t pos
             const int m = first + j;
             if (j == 0 || m % 8 == 0) high = power(m / 8 * 8, n);
             a.turns[i] = axes.scale[x] * (high * low[m % 8]) / (2.0 * M_PI);
-            // else a position times it, or nothing times it, is a NaN
-            require(std::isfinite(a.turns[i] * 0x1p31), "rope: a position times scale and frequency leaves the range of fp64");
+            finite = finite && std::isfinite(a.turns[i] * 0x1p31);   // else a position times it, 0 too, is a NaN
             a.axis[i] = static_cast<uint8_t>(x);
         }
     }
+    require(finite, "rope: a position times scale and frequency leaves the range of fp64");
     const bool interleaved = axes.interleaved != 0;
     const int turned = (interleaved ? 2 * a.pairs + 7 : a.pairs + 7) / 8;
     a.vectors = turned + (a.head_dim - 2 * a.pairs + 7) / 8;
