@@ -620,8 +620,10 @@ int bh_attention_linear(const void* q, int64_t ld_q, const void* k, int64_t ld_k
                 "attention_linear: ld_q, ld_k and ld_v must be multiples of 8, ld_out of 4");
         const int64_t most = int64_t{1} << 24;
         require(ld_q < most && ld_k < most && ld_v < most, "attention_linear: ld_q, ld_k and ld_v must be below 2^24");
-        require(heads > 0 || batch == 0 || !state_out, "attention_linear: state_out without query heads");
-        if (batch * heads == 0 || (seq_len == 0 && !state_out)) return;
+        if (batch * heads == 0 || (seq_len == 0 && !state_out)) {
+            require(heads > 0 || batch == 0 || !state_out, "attention_linear: state_out without query heads");
+            return;
+        }
         if (seq_len > 0) {   // without tokens the state is copied
             require_device_ptr(q, op, "q");
             require_device_ptr(k, op, "k");
@@ -636,11 +638,8 @@ int bh_attention_linear(const void* q, int64_t ld_q, const void* k, int64_t ld_k
                 "attention_linear: q, k and v must be 16-byte, out 8-byte aligned");
         require(aligned(state_in, 16) && aligned(state_out, 16), "attention_linear: a state is not 16-byte aligned");
         require(aligned(log_decay, 4) && aligned(lens, 4), "attention_linear: an operand is not aligned to its type");
-        if (seq_len > 0) {   // a workgroup would write what another one has still to read
-            require(out != q, "attention_linear: out is q");
-            require(out != k, "attention_linear: out is k");
-            require(out != v, "attention_linear: out is v");
-        }
+        if (seq_len > 0 && (out == q || out == k || out == v))   // a workgroup would write what another one has still to read
+            throw Error(std::string("attention_linear: out is ") + (out == q ? "q" : out == k ? "k" : "v"));
         sh.ld_q = ld_q;
         sh.ld_k = ld_k;
         sh.ld_v = ld_v;
