@@ -20,9 +20,9 @@
 // What bounds it: one token of 16 sequences, 32 states of 128 x 128 each, their bytes (14.9 us, 4.5 TB/s). Chunks, the
 // instructions of few waves: at 128 x 128 a chunk takes 2.3 us alone on a CU, two 3.9, where matrix (100, 1600 cycles) and vector
 // instructions (361) of two waves of a SIMD overlap little, and issuing a wave's six direct loads takes 500 to 800 cycles of 6500.
-// Two heads at once take 152 and 430 instead of 200 and 722: 2 x 4096 tokens of 32 / 8 heads of 128 71 us (83 with one), 51 of
-// it the third launch; 65536 tokens of 16 heads of 128 351 us, near its bytes: k and v twice, 106 us of it the first launch
-// (4.9 TB/s), 15 the second; 2 x 300 of 64 heads of 64 16.8 us.
+// Two heads at once take 152 and 430 instead of 200 and 722: 2 x 4096 tokens of 32 / 8 heads of 128 71 to 74 us (83 with one where it
+// took 71), 51 of it the third launch; 65536 tokens of 16 heads of 128 350 to 361 us, bound by bytes: k and v twice, 106 us of it
+// the first launch (4.9 TB/s), 15 the second; 2 x 300 of 64 heads of 64 16.7 us. Ranges are over sixteen runs on several cards.
 #include "common.h"
 
 #include <algorithm>

@@ -160,7 +160,8 @@ void launch_rope(const bh_rope_axes& axes, const int32_t* positions, int64_t pos
     a.vectors = turned + (a.head_dim - 2 * a.pairs + 7) / 8;
     a.items = a.vectors * (q.heads + k.heads);
     // Several rows a workgroup where they are short and enough workgroups remain. Long ones by themselves: 32256 rows of 48 heads
-    // of 128 took 145 us, two to a workgroup 150, five 163; 8192 rows of 32 heads of 72, two to a workgroup, 15.1, four 14.7.
+    // of 128 (384 items) took 145 us, two to a workgroup 150, five 163. 8192 rows of 32 heads of 72 (288) are given two and took 15.1;
+    // four took 14.7, but a limit that allows four of 288 items allows two of 384.
     a.per = static_cast<int>(std::min<int64_t>({16, 1024 / a.pairs, std::max(1, 640 / a.items), std::max<int64_t>(1, rows / 2048)}));
     a.by_pairs = reciprocal(a.pairs);
     a.by_vectors = reciprocal(a.vectors);
