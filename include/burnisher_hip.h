@@ -341,7 +341,8 @@ int64_t bh_attention_linear_workspace_bytes(int64_t batch, int64_t heads, int64_
 typedef struct bh_attention_linear_plan {
     int chunk;            /* tokens a step takes at once; 1: token after token */
     int segments;         /* of a sequence, side by side; above 1 the workspace takes their states */
-    int64_t workgroups;
+    int64_t workgroups;   /* of the launch that writes the outputs; a group's heads take turns in one where, without a
+                           * workspace, the state is updated in place */
 } bh_attention_linear_plan;
 int bh_attention_linear_describe(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len,
                                  int64_t head_dim, int64_t value_dim, int with_workspace, int cus,
